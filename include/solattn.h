@@ -307,6 +307,83 @@ SOLATTN_API int solattn_status_to_host(const int32_t* status, int32_t* host_dst,
  */
 SOLATTN_API int solattn_read_status(int32_t* status, int32_t* value, void* stream);
 
+/*
+ * Attention with a token-exact window and sinks (no counterpart in the reference, whose local and
+ * sink rules work on 64-token blocks).  q and out hold Hq heads, k and v Hkv heads (Hq a multiple
+ * of Hkv; query head h reads K/V head h / (Hq / Hkv)); BF16, element strides as above, out a
+ * contiguous [B, Tq, Hq, D].  Query i has position p = Tk - Tq + i; key j is visible to it iff
+ * j <= p + lookahead (lookahead -1: no bound) and (j > p - window (window 0: no bound) or
+ * j < sink_tokens).  A query that sees no key gives zeros; keys that a query does not see have no
+ * influence on it whatever they hold.  FP32 softmax and sums, P rounded to BF16 for P V.
+ * `workspace`: solattn_window_workspace_bytes() bytes, 16-byte aligned (NULL when that is 0), with
+ * no contents that a call expects.  `status`: a device-accessible int32 word (device memory or
+ * pinned host memory) or NULL; kernels store a SOLATTN device-side code in it and never clear it.
+ */
+SOLATTN_API int solattn_window_attention(const void* q, const void* k, const void* v, int64_t B, int64_t Tq,
+                      int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D,
+                      int64_t q_sB, int64_t q_sT, int64_t q_sH,
+                      int64_t k_sB, int64_t k_sT, int64_t k_sH,
+                      int64_t v_sB, int64_t v_sT, int64_t v_sH,
+                      int64_t window, int64_t lookahead, int64_t sink_tokens, float scale,
+                      void* workspace, int64_t workspace_bytes, void* out, int32_t* status,
+                      void* stream);
+
+/* Workspace bytes of solattn_window_attention, or -1 on an invalid shape. */
+SOLATTN_API int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq,
+                      int64_t Hkv, int64_t D, int64_t window, int64_t lookahead,
+                      int64_t sink_tokens);
+
+/*
+ * Paged K/V cache (no counterpart in the reference).  k_pages and v_pages are contiguous
+ * [pages, Hkv, page_size, D] with page_size 16, 32, 64 or 128: BF16 when k_scale and v_scale are
+ * NULL, else E4M3 codes with one power-of-two scale per (token, head) as E8M0 exponents
+ * [pages, Hkv, page_size] (value = code * 2^(exponent - 127), 255 = NaN).  A call covers B
+ * sequences: token t of sequence b lies in page page_table[b * table_width + t / page_size] at
+ * t % page_size; key_lengths[b] counts its tokens, new ones included; its new tokens are the rows
+ * query_starts[b] .. query_starts[b + 1] - 1 of the packed [N, heads, D] tensors and the last ones
+ * of the sequence.  Rows from query_starts[B] on belong to no sequence.  Page table entries that
+ * no visible key needs are not read and may hold anything.  Values outside their range (a
+ * page, a length, a start) are reported through `status` (as above) and never addressed.
+ *
+ * solattn_paged_attention: the packed queries q [N, Hq, D] (strides q_sT, q_sH) against their
+ * sequences' keys under the visibility rule of solattn_window_attention with p = key_lengths[b] -
+ * (new tokens of b) + i; out is a contiguous [N, Hq, D].  Rows behind the last sequence are left as
+ * they are, or with zero_tail != 0 set to zero.  Workspace as above.
+ */
+SOLATTN_API int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
+                      int64_t q_sT, int64_t q_sH, const void* k_pages, const void* v_pages,
+                      const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size,
+                      const int32_t* page_table, int64_t table_width, const int32_t* key_lengths,
+                      const int32_t* query_starts, int64_t B, int64_t window, int64_t lookahead,
+                      int64_t sink_tokens, float scale, int zero_tail, void* workspace,
+                      int64_t workspace_bytes, void* out, int32_t* status, void* stream);
+
+/* Workspace bytes of solattn_paged_attention, or -1 on an invalid shape. */
+SOLATTN_API int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                      int64_t page_size, int64_t table_width, int64_t window, int64_t lookahead,
+                      int64_t sink_tokens);
+
+/*
+ * Writes the new tokens' K and V rows (packed BF16 [N, Hkv, D], strides k_sT ...) to their places in
+ * the cache.  E4M3: per (token, head) the scale is 2^e with the least integer e in [-127, 127] for
+ * which max|x| <= 448 * 2^e over the row's finite values; code = x * 2^-e rounded to nearest even,
+ * saturating; NaN stays NaN.  Two sequences that write the same page race on it.
+ */
+SOLATTN_API int solattn_cache_write(const void* k, const void* v, int64_t N, int64_t Hkv, int64_t D,
+                      int64_t k_sT, int64_t k_sH, int64_t v_sT, int64_t v_sH, void* k_pages,
+                      void* v_pages, void* k_scale, void* v_scale, int64_t pages,
+                      int64_t page_size, const int32_t* page_table, int64_t table_width,
+                      const int32_t* key_lengths, const int32_t* query_starts, int64_t B,
+                      int32_t* status, void* stream);
+
+/* Reads tokens [0, tokens) of every sequence into contiguous BF16 k and v [B, tokens, Hkv, D], with
+ * zeros behind a sequence's end. */
+SOLATTN_API int solattn_cache_read(const void* k_pages, const void* v_pages, const void* k_scale,
+                      const void* v_scale, int64_t pages, int64_t page_size,
+                      const int32_t* page_table, int64_t table_width, const int32_t* key_lengths,
+                      int64_t B, int64_t Hkv, int64_t D, int64_t tokens, void* k, void* v,
+                      int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,227 @@
+// Shared parts of the paged-cache and windowed attention kernels: the K/V sources (contiguous
+// BTHD tensors, paged BF16 or E4M3 caches), the sequences of a call, the visibility rule, and the
+// E4M3 conversions.
+//
+// A call covers B sequences; sequence b has n new tokens (queries) and L keys, and its query i has
+// position p = L - n + i.  Key j is visible to it iff 0 <= j < L, j <= p + ahead and
+// (j > p - window or j < sinks).  Query heads share K/V heads in groups of G = Hq / Hkv; the rows
+// of a (sequence, K/V head) are its n * G (token, head) pairs, row r = token r / G, head r % G of
+// the group, so that one tile of rows serves every query head of the K/V head.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace solattn {
+
+// Where K and V come from.
+enum KvKind { kStrided = 0, kPagedBf16 = 1, kPagedE4m3 = 2 };
+
+constexpr int kNoBound = 1 << 30;  // window / ahead without a bound (positions stay below 2^30)
+
+struct SeqParams {
+  const __nv_bfloat16* q;
+  int64_t q_sB, q_sT, q_sH;  // element strides; packed (paged) queries have q_sB = 0
+  const uint8_t* k;          // BF16 rows, or E4M3 codes
+  const uint8_t* v;
+  const uint8_t* k_scale;  // E8M0 exponents [pages, Hkv, page_size] (E4M3 caches), else nullptr
+  const uint8_t* v_scale;
+  int64_t k_sB, k_sT, k_sH, v_sB, v_sT, v_sH;  // contiguous sources: element strides
+  // Paged sources: pages [pages, Hkv, page_size, D]; page_table [B, width]; else nullptr.
+  const int32_t* table;
+  const int32_t* lengths;  // keys of each sequence [B]
+  const int32_t* starts;   // query_starts [B + 1]
+  int width, page_shift, pages;
+  __nv_bfloat16* out;  // [tokens, Hq, D], packed
+  float* part;         // partial results of split rows (see rows.cu), or nullptr
+  int32_t* status;     // device-accessible word (pinned host memory) or nullptr
+  int B, N, Hq, Hkv, G, Tq, Tk;  // N: rows of q over all sequences (B * Tq when contiguous)
+  int window, ahead, sinks;
+  int slots, splits, unit;  // row tiles over all sequences; splits of a tile; keys tiles per split
+  int zero_tail;            // write zeros to the rows behind the last sequence
+  float scale_log2;         // softmax scale * log2(e)
+};
+
+struct CacheParams {
+  const __nv_bfloat16* x[2];  // new K and V rows [N, Hkv, D]
+  int64_t sT[2], sH[2];       // element strides
+  uint8_t* pages[2];          // K and V pages [pages, Hkv, page_size, D]
+  uint8_t* scale[2];          // E8M0 exponents [pages, Hkv, page_size], or nullptr
+  const int32_t* table;       // [B, width]
+  const int32_t* lengths;     // [B], the new tokens included
+  const int32_t* starts;      // [B + 1]
+  __nv_bfloat16* y[2];        // read: K and V [B, tokens, Hkv, D]
+  int32_t* status;
+  int B, N, Hkv, width, page_shift, npages, tokens;
+};
+
+// Device-side errors of these kernels go to a word of pinned host memory, shared by all calls on a
+// device: a plain store (any error may win), so that a call without errors touches it never.
+__device__ __forceinline__ void note(int32_t* status, int code) {
+  if (status) *reinterpret_cast<volatile int32_t*>(status) = code;
+}
+
+struct Seq {
+  int b;      // sequence, or -1: the slot holds no rows
+  int tile;   // the slot's row tile within the sequence
+  int n, L;   // new tokens and keys
+  int start;  // first packed token
+};
+
+// Row tiles are numbered so that no prefix sum over the sequences is needed: sequence b's tiles of
+// R rows start at slot first(b) = floor(start_b * G / R) + b.  Since floor(x + y) + 1 >= floor(x) +
+// ceil(y), every sequence has room for its ceil(n G / R) tiles before first(b + 1); the slots in
+// between hold no rows.  One warp finds the last b with first(b) <= slot, 32 probes at a time.
+// Values outside their range are reported and the sequence is left out.
+__device__ __forceinline__ int slot_first(int start, int G, int R, int b) {
+  return (int)((int64_t)start * G / R) + b;
+}
+
+template <int R>
+__device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) {
+  Seq s;
+  if (!p.table) {
+    const int tiles = (p.Tq * p.G + R - 1) / R;  // (Tq * G < 2^31: checked by the host)
+    s.b = slot / tiles;
+    s.tile = slot % tiles;
+    s.n = p.Tq;
+    s.L = p.Tk;
+    s.start = s.b * p.Tq;
+    return s;
+  }
+  int lo = 0, hi = p.B;  // the answer lies in [lo, hi)
+  int start = 0, next = 0;
+  while (true) {
+    // Lane l probes b = lo + l * step.  The first probe (b = lo) always satisfies the condition.
+    const int step = (hi - lo + 31) / 32;
+    const int b = lo + lane * step;
+    const bool in = b < hi;
+    const int st = in ? __ldg(p.starts + b) : 0;
+    const int en = (in && step == 1) ? __ldg(p.starts + b + 1) : 0;
+    const bool le = in && (lane == 0 || slot_first(st, p.G, R, b) <= slot);
+    const uint32_t bal = __ballot_sync(0xffffffffu, le);
+    const int last = 31 - __clz(bal);
+    if (step == 1) {
+      s.b = lo + last;
+      start = __shfl_sync(0xffffffffu, st, last);
+      next = __shfl_sync(0xffffffffu, en, last);
+      break;
+    }
+    lo += last * step;
+    hi = min(hi, lo + step);
+  }
+  s.start = start;
+  s.n = next - start;
+  const bool bad = start < 0 || next < start || next > p.N;
+  if (bad) note(p.status, kStatusBadIndex);
+  s.tile = slot - slot_first(start, p.G, R, s.b);
+  if (bad || s.tile < 0 || (int64_t)s.tile * R >= (int64_t)s.n * p.G) {
+    s.b = -1;
+    s.n = s.L = s.tile = 0;
+    return s;
+  }
+  int L = __ldg(p.lengths + s.b);
+  const int cap = p.width << p.page_shift;
+  if (L < 0 || L > cap) {
+    note(p.status, kStatusBadIndex);
+    L = L < 0 ? 0 : cap;
+  }
+  s.L = L;
+  return s;
+}
+
+// The keys that a query at position pos sees: [lo, hi] and [0, min(sinks - 1, hi)].
+__device__ __forceinline__ int key_high(const SeqParams& p, int L, int pos) {
+  return p.ahead >= kNoBound ? L - 1 : min(L - 1, pos + p.ahead);
+}
+__device__ __forceinline__ int key_low(const SeqParams& p, int pos) {
+  return p.window >= kNoBound ? 0 : max(0, pos - p.window + 1);
+}
+
+// The key tiles (of T keys) that the queries at positions [p0, p1] need: [0, sink) and [from, to).
+struct KeyTiles {
+  int sink, from, to;
+  __device__ __forceinline__ int count() const { return sink + to - from; }
+  // Key tile number i of the list.
+  __device__ __forceinline__ int at(int i) const { return i < sink ? i : from + i - sink; }
+};
+template <int T>
+__device__ __forceinline__ KeyTiles key_tiles(const SeqParams& p, int L, int p0, int p1) {
+  KeyTiles k;
+  const int high = key_high(p, L, p1);  // the last key that any of them sees (or below 0)
+  k.from = k.to = k.sink = 0;
+  if (high < 0) return k;
+  k.from = min(key_low(p, p0), high + 1) / T;  // (a window that starts behind the keys is empty)
+  k.to = high / T + 1;
+  const int sinks = min(p.sinks, high + 1);
+  k.sink = min((sinks + T - 1) / T, k.from);
+  return k;
+}
+
+// Page of the key tile at `key` (page sizes are multiples of the callers' pieces).  A page outside
+// the pool is reported and replaced by page 0, so that every address stays in range.
+__device__ __forceinline__ int page_of(const SeqParams& p, int b, int key) {
+  int page = __ldg(p.table + (int64_t)b * p.width + (key >> p.page_shift));
+  if (page < 0 || page >= p.pages) {
+    note(p.status, kStatusBadIndex);
+    page = 0;
+  }
+  return page;
+}
+
+// Rows behind the last sequence of a packed call: zeros, when the caller asked for them.  Called by
+// all threads of the CTAs `part` of `parts`.
+template <int D>
+__device__ __forceinline__ void zero_tail(const SeqParams& p, int part, int parts) {
+  if (!p.zero_tail || !p.table) return;
+  const int end = __ldg(p.starts + p.B);
+  if (end < 0 || end >= p.N) return;
+  const int64_t chunks = (int64_t)p.Hq * D / 8;  // 16-byte pieces of a token
+  for (int64_t t = (int64_t)end + part; t < p.N; t += parts) {
+    uint4* dst = reinterpret_cast<uint4*>(p.out + t * p.Hq * D);
+    for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------- E4M3 and E8M0
+// 2^(e - 127); 255 is NaN.
+__device__ __forceinline__ float e8m0_value(uint32_t e) {
+  return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7fc00000u : e << 23);
+}
+
+// Two E4M3 codes in the high bytes of the 16-bit halves of x -> the same bits in BF16's fields: a
+// BF16 pair that is 2^-120 times the two values (the formats differ by 120 in exponent bias, and
+// E4M3's subnormals become BF16's).
+__device__ __forceinline__ uint32_t e4m3_fields(uint32_t x) {
+  return ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
+}
+constexpr uint32_t kTwo120x2 = 0x7b807b80u;  // BF16 pair of 2^120
+
+__device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t bf16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
+// One E4M3 code as FP32 (0x7f and 0xff are NaN).
+__device__ __forceinline__ float e4m3_value(uint32_t c) {
+  const uint32_t mag = c & 0x7fu;
+  if (mag == 0x7fu) return __uint_as_float(0x7fc00000u);
+  const float v = __uint_as_float(mag << 20) * __uint_as_float(247u << 23);  // fields, then 2^120
+  return (c & 0x80u) ? -v : v;
+}
+
+// Bytes equal to 0x7f or 0xff (E4M3's NaN) in any of the four: nonzero.
+__device__ __forceinline__ uint32_t e4m3_nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+}  // namespace solattn

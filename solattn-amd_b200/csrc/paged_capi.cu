@@ -1,0 +1,276 @@
+// extern "C" entry points of the windowed and paged attention and of the paged cache (declared in
+// include/solattn.h).  Every argument is checked before the first CUDA call.
+#include <math.h>
+
+#include "../../include/solattn.h"
+#include "paged.cuh"
+
+namespace solattn {
+
+cudaError_t launch_rows(const SeqParams& p, int D, int kv, cudaStream_t stream);
+cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream);
+cudaError_t launch_cache_read(const CacheParams& p, int D, cudaStream_t stream);
+
+}  // namespace solattn
+
+using namespace solattn;
+
+namespace {
+
+constexpr int64_t kMaxKeys = int64_t(1) << 24;  // keys of a sequence, as in the routed entry points
+constexpr int64_t kSms = 148;
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+bool stride_ok(int64_t s) { return s > 0 && s % 8 == 0; }
+int from_cuda(cudaError_t e) { return e == cudaSuccess ? SOLATTN_OK : SOLATTN_ERR_LAUNCH; }
+
+int page_shift_of(int64_t page_size) {
+  for (int s = 4; s <= 7; ++s)
+    if (page_size == (int64_t(1) << s)) return s;
+  return -1;
+}
+
+struct Rule {
+  int64_t window, lookahead, sinks;  // window 0 and lookahead -1: no bound
+};
+bool rule_ok(const Rule& r) {
+  return r.window >= 0 && r.window < kNoBound && r.lookahead >= -1 && r.lookahead < kNoBound &&
+         r.sinks >= 0 && r.sinks < kNoBound;
+}
+
+// How the few-rows kernel divides a call: tiles of 16 rows (slots, see find_seq), and every tile's
+// keys over `splits` CTAs of at least `unit` 16-key chunks.
+struct Split {
+  int64_t slots, splits, unit;
+};
+Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t cap, bool paged,
+                 const Rule& r) {
+  Split s;
+  const int64_t G = Hq / Hkv;
+  s.slots = paged ? N * G / 16 + B : B * cdiv(Tq * G, 16);
+  int64_t keys = cap;
+  if (r.window > 0 && r.lookahead >= 0) {
+    const int64_t span = r.window + r.lookahead + r.sinks + 16 + 48;
+    if (span < keys) keys = span;
+  }
+  const int64_t chunks = cdiv(keys, 16) + 2;
+  int64_t unit = cdiv(chunks * s.slots * Hkv, kSms * 2 * 4);
+  if (unit < 16) unit = 16;
+  if (unit > 128) unit = 128;
+  if (unit < cdiv(chunks, 64)) unit = cdiv(chunks, 64);
+  s.unit = unit;
+  s.splits = cdiv(chunks, unit);
+  return s;
+}
+int64_t split_bytes(const Split& s, int64_t Hkv, int64_t D) {
+  return s.splits > 1 ? s.slots * Hkv * s.splits * 16 * (D + 2) * 4 : 0;
+}
+
+int check_heads(int64_t Hq, int64_t Hkv, int64_t D) {
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq > 65535) return SOLATTN_ERR_ARG;
+  if (D != 64 && D != 128) return SOLATTN_ERR_UNSUPPORTED;
+  return SOLATTN_OK;
+}
+int check_window(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hkv, int64_t D, const Rule& r) {
+  if (B <= 0 || Tq <= 0 || Tk <= 0) return SOLATTN_ERR_ARG;
+  const int rc = check_heads(Hq, Hkv, D);
+  if (rc) return rc;
+  if (!rule_ok(r) || Tq > kMaxKeys || Tk > kMaxKeys) return SOLATTN_ERR_ARG;
+  if (B * Tq > (int64_t(1) << 31) / (Hq / Hkv) - 1 || B > (1 << 24)) return SOLATTN_ERR_ARG;
+  return SOLATTN_OK;
+}
+int check_paged(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size, int64_t width,
+                const Rule& r) {
+  if (N <= 0 || B <= 0 || width <= 0) return SOLATTN_ERR_ARG;
+  const int rc = check_heads(Hq, Hkv, D);
+  if (rc) return rc;
+  if (page_shift_of(page_size) < 0) return SOLATTN_ERR_UNSUPPORTED;
+  if (!rule_ok(r) || width * page_size > kMaxKeys) return SOLATTN_ERR_ARG;
+  if (N > (int64_t(1) << 31) / (Hq / Hkv) - 1 - (1 << 24) || B > (1 << 24)) return SOLATTN_ERR_ARG;
+  return SOLATTN_OK;
+}
+
+void set_rule(SeqParams& p, const Rule& r, float scale) {
+  p.window = r.window == 0 ? kNoBound : (int)r.window;
+  p.ahead = r.lookahead < 0 ? kNoBound : (int)r.lookahead;
+  p.sinks = (int)r.sinks;
+  p.scale_log2 = scale * 1.4426950408889634f;
+}
+
+int run(SeqParams& p, int64_t D, int kv, const Split& s, void* workspace, int64_t workspace_bytes,
+        void* stream) {
+  if (s.slots * p.Hkv * s.splits >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  if (split_bytes(s, p.Hkv, D) > workspace_bytes) return SOLATTN_ERR_ARG;
+  if (s.splits > 1 && (!workspace || !aligned16(workspace))) return SOLATTN_ERR_ARG;
+  p.slots = (int)s.slots;
+  p.splits = (int)s.splits;
+  p.unit = (int)s.unit;
+  p.part = static_cast<float*>(workspace);
+  return from_cuda(launch_rows(p, (int)D, kv, static_cast<cudaStream_t>(stream)));
+}
+
+int cache_params(CacheParams& p, const void* k_pages, const void* v_pages, const void* k_scale,
+                 const void* v_scale, int64_t pages, int64_t page_size, int64_t B, int64_t Hkv, int64_t D,
+                 const int32_t* page_table, int64_t width, const int32_t* key_lengths, int32_t* status) {
+  if (!k_pages || !v_pages || (k_scale == nullptr) != (v_scale == nullptr)) return SOLATTN_ERR_ARG;
+  if (!page_table || !key_lengths || B <= 0 || B > (1 << 24) || Hkv <= 0 || Hkv > 65535 || pages <= 0 ||
+      pages > 0x7fffffff || width <= 0)
+    return SOLATTN_ERR_ARG;
+  if (D != 64 && D != 128) return SOLATTN_ERR_UNSUPPORTED;
+  if (page_shift_of(page_size) < 0) return SOLATTN_ERR_UNSUPPORTED;
+  if (width * page_size > kMaxKeys || !aligned16(k_pages) || !aligned16(v_pages)) return SOLATTN_ERR_ARG;
+  p.pages[0] = static_cast<uint8_t*>(const_cast<void*>(k_pages));
+  p.pages[1] = static_cast<uint8_t*>(const_cast<void*>(v_pages));
+  p.scale[0] = static_cast<uint8_t*>(const_cast<void*>(k_scale));
+  p.scale[1] = static_cast<uint8_t*>(const_cast<void*>(v_scale));
+  p.table = page_table;
+  p.lengths = key_lengths;
+  p.status = status;
+  p.B = (int)B;
+  p.Hkv = (int)Hkv;
+  p.width = (int)width;
+  p.page_shift = page_shift_of(page_size);
+  p.npages = (int)pages;
+  return SOLATTN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hkv,
+                                       int64_t D, int64_t window, int64_t lookahead, int64_t sink_tokens) {
+  const Rule r{window, lookahead, sink_tokens};
+  if (check_window(B, Tq, Tk, Hq, Hkv, D, r)) return -1;
+  return split_bytes(rows_split(B * Tq, B, Hq, Hkv, Tq, Tk, false, r), Hkv, D);
+}
+
+int solattn_window_attention(const void* q, const void* k, const void* v, int64_t B, int64_t Tq, int64_t Tk,
+                             int64_t Hq, int64_t Hkv, int64_t D, int64_t q_sB, int64_t q_sT, int64_t q_sH,
+                             int64_t k_sB, int64_t k_sT, int64_t k_sH, int64_t v_sB, int64_t v_sT,
+                             int64_t v_sH, int64_t window, int64_t lookahead, int64_t sink_tokens, float scale,
+                             void* workspace, int64_t workspace_bytes, void* out, int32_t* status,
+                             void* stream) {
+  const Rule r{window, lookahead, sink_tokens};
+  const int rc = check_window(B, Tq, Tk, Hq, Hkv, D, r);
+  if (rc) return rc;
+  if (!q || !k || !v || !out || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+    return SOLATTN_ERR_ARG;
+  const int64_t strides[9] = {q_sB, q_sT, q_sH, k_sB, k_sT, k_sH, v_sB, v_sT, v_sH};
+  for (int i = 0; i < 9; ++i)
+    if (!stride_ok(strides[i])) return SOLATTN_ERR_ARG;
+  if (!(scale > 0.f) || !isfinite(scale)) return SOLATTN_ERR_ARG;
+  SeqParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.k = static_cast<const uint8_t*>(k);
+  p.v = static_cast<const uint8_t*>(v);
+  p.q_sB = q_sB, p.q_sT = q_sT, p.q_sH = q_sH;
+  p.k_sB = k_sB, p.k_sT = k_sT, p.k_sH = k_sH;
+  p.v_sB = v_sB, p.v_sT = v_sT, p.v_sH = v_sH;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.status = status;
+  p.B = (int)B;
+  p.N = (int)(B * Tq);
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.G = (int)(Hq / Hkv);
+  p.Tq = (int)Tq;
+  p.Tk = (int)Tk;
+  set_rule(p, r, scale);
+  return run(p, D, kStrided, rows_split(B * Tq, B, Hq, Hkv, Tq, Tk, false, r), workspace, workspace_bytes,
+             stream);
+}
+
+int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                      int64_t page_size, int64_t table_width, int64_t window,
+                                      int64_t lookahead, int64_t sink_tokens) {
+  const Rule r{window, lookahead, sink_tokens};
+  if (check_paged(N, B, Hq, Hkv, D, page_size, table_width, r)) return -1;
+  return split_bytes(rows_split(N, B, Hq, Hkv, 0, table_width * page_size, true, r), Hkv, D);
+}
+
+int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_sT,
+                            int64_t q_sH, const void* k_pages, const void* v_pages, const void* k_scale,
+                            const void* v_scale, int64_t pages, int64_t page_size, const int32_t* page_table,
+                            int64_t table_width, const int32_t* key_lengths, const int32_t* query_starts,
+                            int64_t B, int64_t window, int64_t lookahead, int64_t sink_tokens, float scale,
+                            int zero_tail, void* workspace, int64_t workspace_bytes, void* out,
+                            int32_t* status, void* stream) {
+  const Rule r{window, lookahead, sink_tokens};
+  const int rc = check_paged(N, B, Hq, Hkv, D, page_size, table_width, r);
+  if (rc) return rc;
+  if (!q || !k_pages || !v_pages || !page_table || !key_lengths || !query_starts || !out ||
+      (k_scale == nullptr) != (v_scale == nullptr) || pages <= 0 || pages > 0x7fffffff)
+    return SOLATTN_ERR_ARG;
+  if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
+      (k_scale && (!aligned16(k_scale) || !aligned16(v_scale))) || !stride_ok(q_sT) || !stride_ok(q_sH))
+    return SOLATTN_ERR_ARG;
+  if (!(scale > 0.f) || !isfinite(scale)) return SOLATTN_ERR_ARG;
+  SeqParams p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_sT = q_sT;
+  p.q_sH = q_sH;
+  p.k = static_cast<const uint8_t*>(k_pages);
+  p.v = static_cast<const uint8_t*>(v_pages);
+  p.k_scale = static_cast<const uint8_t*>(k_scale);
+  p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.table = page_table;
+  p.lengths = key_lengths;
+  p.starts = query_starts;
+  p.width = (int)table_width;
+  p.page_shift = page_shift_of(page_size);
+  p.pages = (int)pages;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.status = status;
+  p.B = (int)B;
+  p.N = (int)N;
+  p.Hq = (int)Hq;
+  p.Hkv = (int)Hkv;
+  p.G = (int)(Hq / Hkv);
+  p.zero_tail = zero_tail;
+  set_rule(p, r, scale);
+  return run(p, D, k_scale ? kPagedE4m3 : kPagedBf16,
+             rows_split(N, B, Hq, Hkv, 0, table_width * page_size, true, r), workspace, workspace_bytes,
+             stream);
+}
+
+int solattn_cache_write(const void* k, const void* v, int64_t N, int64_t Hkv, int64_t D, int64_t k_sT,
+                        int64_t k_sH, int64_t v_sT, int64_t v_sH, void* k_pages, void* v_pages, void* k_scale,
+                        void* v_scale, int64_t pages, int64_t page_size, const int32_t* page_table,
+                        int64_t table_width, const int32_t* key_lengths, const int32_t* query_starts,
+                        int64_t B, int32_t* status, void* stream) {
+  CacheParams p = {};
+  const int rc = cache_params(p, k_pages, v_pages, k_scale, v_scale, pages, page_size, B, Hkv, D, page_table,
+                              table_width, key_lengths, status);
+  if (rc) return rc;
+  if (!k || !v || !query_starts || N <= 0 || !aligned16(k) || !aligned16(v) || !stride_ok(k_sT) ||
+      !stride_ok(k_sH) || !stride_ok(v_sT) || !stride_ok(v_sH))
+    return SOLATTN_ERR_ARG;
+  if (N > 0x7fffffff || cdiv(N * Hkv * (D / 8), 256) >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  p.x[0] = static_cast<const __nv_bfloat16*>(k);
+  p.x[1] = static_cast<const __nv_bfloat16*>(v);
+  p.sT[0] = k_sT, p.sT[1] = v_sT;
+  p.sH[0] = k_sH, p.sH[1] = v_sH;
+  p.starts = query_starts;
+  p.N = (int)N;
+  return from_cuda(launch_cache_write(p, (int)D, static_cast<cudaStream_t>(stream)));
+}
+
+int solattn_cache_read(const void* k_pages, const void* v_pages, const void* k_scale, const void* v_scale,
+                       int64_t pages, int64_t page_size, const int32_t* page_table, int64_t table_width,
+                       const int32_t* key_lengths, int64_t B, int64_t Hkv, int64_t D, int64_t tokens, void* k,
+                       void* v, int32_t* status, void* stream) {
+  CacheParams p = {};
+  const int rc = cache_params(p, k_pages, v_pages, k_scale, v_scale, pages, page_size, B, Hkv, D, page_table,
+                              table_width, key_lengths, status);
+  if (rc) return rc;
+  if (!k || !v || !aligned16(k) || !aligned16(v) || tokens <= 0 || tokens > kMaxKeys) return SOLATTN_ERR_ARG;
+  if (cdiv(B * tokens * Hkv, 256) * (D / 8) >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  p.y[0] = static_cast<__nv_bfloat16*>(k);
+  p.y[1] = static_cast<__nv_bfloat16*>(v);
+  p.tokens = (int)tokens;
+  return from_cuda(launch_cache_read(p, (int)D, static_cast<cudaStream_t>(stream)));
+}
+
+}  // extern "C"

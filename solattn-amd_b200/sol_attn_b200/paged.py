@@ -1,0 +1,258 @@
+"""A paged K/V cache: writing new tokens, attention over it, and reading sequences back.
+
+A streaming (chunk by chunk) model keeps the K and V of its past tokens in pages of 16 to 128 tokens,
+``PagedKVCache``, in BF16 or in E4M3 with one power-of-two scale per (token, head).  Which pages hold
+which sequence, and which rows of the packed new tokens are whose, says a ``PagedPlan``: one plan
+serves ``cache_write``, ``paged_attention`` and ``cache_read`` of a step.  None of this has a
+counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+from .attention import _is_b200, _nonnegative_integer
+from .status import monitor
+from .window import aligned, check_inputs, check_rule, check_scale, workspace
+
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+@dataclass(frozen=True)
+class PagedKVCache:
+    """K and V pages [pages, heads, page_size, D], contiguous, on one device.
+
+    BF16, or ``torch.float8_e4m3fn`` with the scales ``k_scale`` / ``v_scale`` [pages, heads,
+    page_size] as ``torch.float8_e8m0fnu``: the value of a code is code * scale of its (token, head).
+    """
+
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: Optional[torch.Tensor] = None
+    v_scale: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        xs = [self.k, self.v] + [s for s in (self.k_scale, self.v_scale) if s is not None]
+        if (self.k.ndim != 4 or self.k.shape != self.v.shape or self.k.dtype != self.v.dtype
+                or any(n <= 0 for n in self.k.shape)):
+            raise ValueError("K and V pages must have matching [pages, heads, page_size, D] shapes and types")
+        if self.k.shape[2] not in PAGE_SIZES:
+            raise ValueError("page_size must be 16, 32, 64 or 128")
+        if self.k.shape[3] not in (64, 128):
+            raise ValueError("Only head dimensions 64 and 128 are implemented")
+        if self.k.dtype == torch.float8_e4m3fn:
+            if any(s is None or s.dtype != torch.float8_e8m0fnu or s.shape != self.k.shape[:3]
+                   for s in (self.k_scale, self.v_scale)):
+                raise ValueError("E4M3 pages need float8_e8m0fnu scales [pages, heads, page_size]")
+        elif self.k.dtype != torch.bfloat16 or self.k_scale is not None or self.v_scale is not None:
+            raise ValueError("Cache pages are BF16 without scales or float8_e4m3fn with scales")
+        if any(not x.is_contiguous() or x.device != self.k.device for x in xs):
+            raise ValueError("Cache tensors must be contiguous and on one device")
+        if any(x.data_ptr() % 16 for x in xs):
+            raise ValueError("Cache tensors must start on 16-byte boundaries")
+        # What every launch passes on: page and scale addresses, pages, page size.
+        object.__setattr__(self, "_args", (
+            self.k.data_ptr(), self.v.data_ptr(),
+            None if self.k_scale is None else self.k_scale.data_ptr(),
+            None if self.v_scale is None else self.v_scale.data_ptr(),
+            self.k.shape[0], self.k.shape[2]))
+
+    @classmethod
+    def create(cls, pages, heads, head_dim, *, page_size=64, dtype=torch.bfloat16, device="cuda"):
+        """An empty (zero) cache of ``pages`` pages."""
+        for name, n in (("pages", pages), ("heads", heads)):
+            _nonnegative_integer(name, n)
+            if n == 0:
+                raise ValueError(f"{name} must be positive")
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise ValueError("Cache pages are BF16 without scales or float8_e4m3fn with scales")
+        shape = (pages, heads, page_size, head_dim)
+        one = 2 if dtype == torch.bfloat16 else 1
+        k, v = (torch.zeros(shape[:3] + (one * head_dim,), dtype=torch.uint8, device=device).view(dtype)
+                for _ in range(2))
+        if one == 2:
+            return cls(k, v)
+        ks, vs = (torch.zeros(shape[:3], dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+                  for _ in range(2))
+        return cls(k, v, ks, vs)
+
+    @property
+    def pages(self):
+        return self.k.shape[0]
+
+    @property
+    def heads(self):
+        return self.k.shape[1]
+
+    @property
+    def page_size(self):
+        return self.k.shape[2]
+
+    @property
+    def head_dim(self):
+        return self.k.shape[3]
+
+
+@dataclass(frozen=True)
+class PagedPlan:
+    """Where the tokens of the call's sequences are (int32 tensors on one device).
+
+    Token t of sequence b lies in page ``page_table[b, t // page_size]``; ``key_lengths[b]`` counts
+    its tokens, the new ones included; its new tokens are rows ``query_starts[b]`` to
+    ``query_starts[b + 1] - 1`` of the packed tensors and the sequence's last.  Page table entries
+    of pages that no visible key needs may hold anything (a page given back, -1).  The tensors may
+    be changed in place between calls (a captured graph reads their contents at each replay).
+    """
+
+    page_table: torch.Tensor
+    key_lengths: torch.Tensor
+    query_starts: torch.Tensor
+
+    def __post_init__(self):
+        t, n, s = self.page_table, self.key_lengths, self.query_starts
+        if any(x.dtype != torch.int32 or not x.is_contiguous() or x.device != t.device for x in (t, n, s)):
+            raise ValueError("Plan tensors must be contiguous int32 tensors on one device")
+        if t.ndim != 2 or 0 in t.shape or n.shape != t.shape[:1] or s.shape != (t.shape[0] + 1,):
+            raise ValueError("A plan holds page_table [B, width], key_lengths [B] and query_starts [B + 1]")
+
+    @classmethod
+    def create(cls, page_table, key_lengths, query_starts, *, page_size=64, pages=None):
+        """Construct on CPU, with every value checked, and transfer once with ``to``."""
+        xs = (page_table, key_lengths, query_starts)
+        if any(not isinstance(x, torch.Tensor) or x.device.type != "cpu" for x in xs):
+            raise ValueError("PagedPlan.create takes CPU tensors")
+        if page_size not in PAGE_SIZES:
+            raise ValueError("page_size must be 16, 32, 64 or 128")
+        plan = cls(*(x.clone().contiguous() for x in xs))
+        if int(query_starts[0]) != 0 or bool((query_starts[1:] < query_starts[:-1]).any()):
+            raise ValueError("query_starts must begin with 0 and not decrease")
+        if bool((key_lengths < 0).any()) or bool((key_lengths > page_table.shape[1] * page_size).any()):
+            raise ValueError("key_lengths must fit in the page table")
+        if bool((query_starts[1:] - query_starts[:-1] > key_lengths).any()):
+            raise ValueError("A sequence has more new tokens than keys")
+        if pages is not None and bool((page_table >= pages).any()):
+            raise ValueError("page_table names a page outside the cache")
+        return plan
+
+    def to(self, device):
+        return PagedPlan(*(x.to(device) for x in (self.page_table, self.key_lengths, self.query_starts)))
+
+
+def _check(cache, plan, *xs):
+    """Checks shared by the operators; returns the device."""
+    if not isinstance(cache, PagedKVCache) or not isinstance(plan, PagedPlan):
+        raise ValueError("A PagedKVCache and a PagedPlan are required")
+    device = cache.k.device
+    if device.type != "cuda" or any(x.device != device for x in xs) or not _is_b200(device):
+        raise ValueError("The sm_100a backend requires the cache and Q/K/V on the same NVIDIA B200 CUDA GPU")
+    if plan.page_table.device != device:
+        raise ValueError("Transfer the plan to the cache's device first")
+    return device
+
+
+def _on(device, fn, *args):
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return fn(*args)
+    return fn(*args)
+
+
+def cache_write(cache, plan, k, v):
+    """Write the new tokens' rows ``k``, ``v`` (packed BF16 [N, heads, D]) to their places.
+
+    E4M3 caches: each (token, head) row is scaled by the least power of two under which its largest
+    finite value is at most 448, and rounded once, to nearest even; infinities saturate, NaN stays.
+    Rows behind the last sequence are ignored.  Two sequences that write the same page race on it.
+    """
+    if k.ndim != 3 or k.shape != v.shape or 0 in k.shape:
+        raise ValueError("K/V must have matching nonempty [tokens, heads, D] shapes")
+    check_inputs(k, v)
+    device = _check(cache, plan, k, v)
+    if k.shape[1:] != (cache.heads, cache.head_dim):
+        raise ValueError("K/V heads and dimension must match the cache")
+    _on(device, _write, cache, plan, k, v)
+
+
+def _write(cache, plan, k, v):
+    k, v = aligned(k), aligned(v)
+    N, H, D = k.shape
+    B, width = plan.page_table.shape
+    word = monitor(k.device).word()
+    rc = _lib.load().solattn_cache_write(
+        k.data_ptr(), v.data_ptr(), N, H, D, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        *cache._args, plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(),
+        plan.query_starts.data_ptr(), B, word, torch.cuda.current_stream(k.device).cuda_stream)
+    _lib.check(rc, "solattn_cache_write")
+
+
+def cache_read(cache, plan, tokens):
+    """K and V of tokens [0, ``tokens``) of every sequence as BF16 [B, tokens, heads, D].
+
+    Zeros behind a sequence's end.  The tensors suit ``sol_attention`` and ``window_attention``.
+    """
+    if type(tokens) is not int or not 0 < tokens <= 1 << 24:
+        raise ValueError("tokens must be a positive integer")
+    device = _check(cache, plan)
+    return _on(device, _read, cache, plan, tokens)
+
+
+def _read(cache, plan, tokens):
+    B, width = plan.page_table.shape
+    device = cache.k.device
+    word = monitor(device).word()
+    k, v = (torch.empty((B, tokens, cache.heads, cache.head_dim), dtype=torch.bfloat16, device=device)
+            for _ in range(2))
+    rc = _lib.load().solattn_cache_read(
+        *cache._args, plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(), B, cache.heads,
+        cache.head_dim, tokens, k.data_ptr(), v.data_ptr(), word,
+        torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, "solattn_cache_read")
+    return k, v
+
+
+def paged_attention(q, cache, plan, *, window=None, lookahead=0, sink_tokens=0, scale=None, out=None):
+    """Attention of the packed new tokens ``q`` [N, Hq, D] over their sequences' cached keys.
+
+    The keys of the new tokens are in the cache already (``cache_write`` comes first).  Query i of a
+    sequence with n new tokens and L keys has position p = L - n + i and sees key j iff
+    j <= p + ``lookahead`` (None: all, so that a chunk's tokens see each other) and (j > p - ``window``
+    (None: all) or j < ``sink_tokens``).  Hq is a multiple of the cache's heads.  A query that sees no
+    key gives zeros; keys that a query does not see have no influence on it whatever they hold.
+    Rows behind the last sequence are zero in a new output and left as they are in ``out`` (BF16,
+    contiguous, shaped like ``q``).
+    """
+    if q.ndim != 3 or 0 in q.shape:
+        raise ValueError("Q must be a nonempty packed [tokens, heads, D] tensor")
+    check_inputs(q)
+    device = _check(cache, plan, q)
+    if q.shape[2] != cache.head_dim or q.shape[1] % cache.heads != 0:
+        raise ValueError("Q's dimension must match the cache and its heads be a multiple of the cache's")
+    scale = check_scale(scale, q.shape[2])
+    rule = check_rule(window, lookahead, sink_tokens)
+    if out is not None and (out.dtype != torch.bfloat16 or out.device != device or out.shape != q.shape
+                            or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
+    return _on(device, _attend, q, cache, plan, rule, scale, out)
+
+
+def _attend(q, cache, plan, rule, scale, out):
+    q = aligned(q)
+    N, Hq, D = q.shape
+    B, width = plan.page_table.shape
+    fresh = out is None
+    word = monitor(q.device).word()
+    keep, ws, size = workspace("solattn_paged_workspace_bytes",
+                               (N, B, Hq, cache.heads, D, cache.page_size, width, *rule), q.device)
+    if fresh:
+        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
+    rc = _lib.load().solattn_paged_attention(
+        q.data_ptr(), N, Hq, cache.heads, D, q.stride(0), q.stride(1), *cache._args,
+        plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(), plan.query_starts.data_ptr(), B,
+        *rule, scale, int(fresh), ws, size, out.data_ptr(), word,
+        torch.cuda.current_stream(q.device).cuda_stream)
+    _lib.check(rc, "solattn_paged_attention")
+    return out

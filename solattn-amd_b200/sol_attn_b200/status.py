@@ -12,6 +12,11 @@ looked at
 * in ``SolStats.density()`` and :func:`check_device_errors`, which wait for every pending slot
   (both synchronise anyway).
 
+The paged-cache and windowed operators use one more word per device, in pinned host memory: their
+kernels store a code straight into it when something is wrong and touch it never otherwise, so
+that a call pays nothing for it and may be captured into a CUDA graph.  It is looked at in the same
+two places (``StatusMonitor.check_word``; a wait first synchronises the device).
+
 So an error surfaces at the latest on the next call or the next synchronising read, and a
 production call pays one 4-byte device-to-host copy, never a synchronisation.  The reference's
 kernels report nothing of the kind; this is the negative-code path of the C ABI
@@ -56,6 +61,26 @@ class StatusMonitor:
         self.pending = collections.deque()
         self.next = 0
         self.lock = threading.Lock()
+        # The sticky word of the paged and windowed operators (see the module docstring).
+        self.sticky = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.sticky_word = self.sticky.numpy()
+        self.sticky_ptr = self.sticky.data_ptr()
+        self.sticky_used = False
+
+    def word(self) -> int:
+        """The sticky word's address, for a call that is about to be launched; first raises for
+        an earlier call's error.  Makes no CUDA call."""
+        self.sticky_used = True
+        if self.sticky_word[0]:
+            self.check_word()
+        return self.sticky_ptr
+
+    def check_word(self) -> None:
+        """Raise for a code in the sticky word, and clear it."""
+        value = int(self.sticky_word[0])
+        if value:
+            self.sticky_word[0] = 0
+            raise DeviceError(value)
 
     def record(self, status_ptr: int, stream: torch.cuda.Stream) -> None:
         """Enqueue the copy of the device word at ``status_ptr`` on ``stream``.  A slot is
@@ -78,6 +103,10 @@ class StatusMonitor:
         """Read the completed slots (every pending slot when ``wait``); raise on a nonzero word."""
         with self.lock:
             self._take(wait=wait, limit=None)
+        if self.sticky_used:
+            if wait:
+                torch.cuda.synchronize(self.device_index)
+            self.check_word()
 
     def _take(self, wait: bool, limit) -> None:
         first_error = 0

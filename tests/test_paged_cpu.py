@@ -1,0 +1,174 @@
+"""Refusals and host-side contracts of the windowed and paged operators, without a GPU."""
+
+import pytest
+import torch
+
+from sol_attn_b200 import (PagedKVCache, PagedPlan, _lib, cache_read, cache_write, paged_attention,
+                           window_attention)
+
+BF16 = torch.bfloat16
+
+
+def _qkv(B=1, Tq=4, Tk=9, Hq=4, Hkv=2, D=64):
+    return (torch.zeros((B, Tq, Hq, D), dtype=BF16), torch.zeros((B, Tk, Hkv, D), dtype=BF16),
+            torch.zeros((B, Tk, Hkv, D), dtype=BF16))
+
+
+def _plan(B=2, width=3):
+    return PagedPlan(torch.zeros((B, width), dtype=torch.int32), torch.ones(B, dtype=torch.int32),
+                     torch.arange(B + 1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("change,msg", [
+    (lambda q, k, v: (q[0], k, v), "rank-4"),
+    (lambda q, k, v: (q, k[:, :3], v), "shapes must agree"),
+    (lambda q, k, v: (q[:, :, :3], k, v), "multiple"),
+    (lambda q, k, v: (q[:, :0], k, v), "nonempty"),
+    (lambda q, k, v: (q.float(), k, v), "Only BF16"),
+    (lambda q, k, v: (q[..., :32], k[..., :32], v[..., :32]), "head dimensions"),
+    (lambda q, k, v: (q, k.transpose(1, 3).contiguous().transpose(1, 3), v), "contiguous head"),
+    (lambda q, k, v: (q.requires_grad_(), k, v), "Inference only"),
+    (lambda q, k, v: (q[:1].expand(1, 4, 4, 64), k[:, :1].expand(1, 9, 2, 64), v), "positive strides"),
+    (lambda q, k, v: (q, k, v), "B200"),
+])
+def test_window_attention_refuses(change, msg):
+    with pytest.raises(ValueError, match=msg):
+        window_attention(*change(*_qkv()))
+
+
+@pytest.mark.parametrize("rule,msg", [
+    (dict(window=0), "window"), (dict(window=-1), "window"), (dict(window=1.5), "window"),
+    (dict(window=1 << 30), "window"), (dict(lookahead=-1), "lookahead"), (dict(lookahead=True), "lookahead"),
+    (dict(sink_tokens=-1), "sink_tokens"), (dict(sink_tokens=None), "sink_tokens"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+])
+def test_rules_are_checked(rule, msg):
+    with pytest.raises(ValueError, match=msg):
+        window_attention(*_qkv(), **rule)
+
+
+def test_cache_construction():
+    c = PagedKVCache.create(3, 2, 64, page_size=16, device="cpu")
+    assert (c.pages, c.heads, c.page_size, c.head_dim) == (3, 2, 16, 64) and c.k_scale is None
+    c = PagedKVCache.create(3, 2, 128, dtype=torch.float8_e4m3fn, device="cpu")
+    assert c.k.dtype == torch.float8_e4m3fn and c.k_scale.shape == (3, 2, 64)
+    assert not c.k.float().any()
+    for bad, msg in (((0, 2, 64), "pages"), ((3, 0, 64), "heads"), ((3, 2, 96), "head dimensions")):
+        with pytest.raises(ValueError, match=msg):
+            PagedKVCache.create(*bad, device="cpu")
+    with pytest.raises(ValueError, match="page_size"):
+        PagedKVCache.create(3, 2, 64, page_size=48, device="cpu")
+    with pytest.raises(ValueError, match="BF16"):
+        PagedKVCache.create(3, 2, 64, dtype=torch.float16, device="cpu")
+    with pytest.raises(ValueError, match="scales"):
+        PagedKVCache(c.k, c.v)
+    with pytest.raises(ValueError, match="matching"):
+        PagedKVCache(c.k, c.v[:2], c.k_scale, c.v_scale)
+    x = torch.zeros((3, 2, 64, 64), dtype=BF16)
+    with pytest.raises(ValueError, match="BF16 without"):
+        PagedKVCache(x, x, c.k_scale, c.v_scale)
+    with pytest.raises(ValueError, match="contiguous"):
+        PagedKVCache(x.transpose(0, 1).contiguous().transpose(0, 1), x)
+
+
+def test_plan_construction():
+    t = torch.tensor([[0, 1], [2, -1]], dtype=torch.int32)
+    n, s = torch.tensor([20, 16], dtype=torch.int32), torch.tensor([0, 3, 4], dtype=torch.int32)
+    PagedPlan.create(t, n, s, page_size=16, pages=3)
+    for args, kw, msg in [
+            ((t.long(), n, s), {}, "int32"), ((t, n[:1], s), {}, "page_table"), ((t, n, s[:2]), {}, "page_table"),
+            ((t, n, s), dict(page_size=8), "page_size"), ((t, n, s + 1), dict(page_size=16), "begin"),
+            ((t, n, torch.tensor([0, 3, 2], dtype=torch.int32)), dict(page_size=16), "decrease"),
+            ((t, n + 20, s), dict(page_size=16), "fit"), ((t, n - 17, s), dict(page_size=16), "fit"),
+            ((t, torch.tensor([2, 16], dtype=torch.int32), s), dict(page_size=16), "more new tokens"),
+            ((t, n, s), dict(page_size=16, pages=2), "outside"), ((t.to("meta"), n, s), {}, "CPU")]:
+        with pytest.raises(ValueError, match=msg):
+            PagedPlan.create(*args, **kw)
+
+
+def test_paged_operators_refuse():
+    c, p = PagedKVCache.create(3, 2, 64, page_size=16, device="cpu"), _plan()
+    q, k = torch.zeros((2, 4, 64), dtype=BF16), torch.zeros((2, 2, 64), dtype=BF16)
+    with pytest.raises(ValueError, match="packed"):
+        paged_attention(q[0], c, p)
+    with pytest.raises(ValueError, match="Only BF16"):
+        paged_attention(q.float(), c, p)
+    with pytest.raises(ValueError, match="PagedKVCache"):
+        paged_attention(q, None, p)
+    with pytest.raises(ValueError, match="B200"):
+        paged_attention(q, c, p)
+    with pytest.raises(ValueError, match="matching"):
+        cache_write(c, p, k, k[:1])
+    with pytest.raises(ValueError, match="B200"):
+        cache_write(c, p, k, k)
+    with pytest.raises(ValueError, match="tokens"):
+        cache_read(c, p, 0)
+    with pytest.raises(ValueError, match="B200"):
+        cache_read(c, p, 5)
+
+
+def _window(**over):
+    a = dict(q=16, k=16, v=16, B=1, Tq=4, Tk=64, Hq=4, Hkv=2, D=64, strides=(4096, 64, 64), window=0, ahead=-1,
+             sinks=0, scale=0.125, ws=None, size=0, out=16)
+    a.update(over)
+    return _lib.load().solattn_window_attention(
+        a["q"], a["k"], a["v"], a["B"], a["Tq"], a["Tk"], a["Hq"], a["Hkv"], a["D"], *a["strides"],
+        *a["strides"], *a["strides"], a["window"], a["ahead"], a["sinks"], a["scale"], a["ws"], a["size"],
+        a["out"], None, None)
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(q=None), -1), (dict(q=8), -1), (dict(out=8), -1), (dict(B=0), -1), (dict(Tk=0), -1), (dict(D=96), -2),
+    (dict(Hq=5), -1), (dict(strides=(4096, 63, 64)), -1), (dict(window=-1), -1), (dict(ahead=-2), -1),
+    (dict(sinks=-1), -1), (dict(scale=0.0), -1), (dict(scale=float("inf")), -1), (dict(Tk=1 << 25), -1),
+    (dict(Tk=100000), -1),  # (needs a workspace)
+])
+def test_window_entry_point_rejects(bad, code):
+    assert _window(**bad) == code
+
+
+def _paged(**over):
+    a = dict(q=16, N=2, Hq=4, Hkv=2, D=64, qs=(256, 64), k=16, v=16, ks=None, vs=None, pages=4, page_size=16,
+             table=16, width=3, lengths=16, starts=16, B=2, window=0, ahead=-1, sinks=0, scale=0.125, ws=None,
+             size=0, out=16)
+    a.update(over)
+    return _lib.load().solattn_paged_attention(
+        a["q"], a["N"], a["Hq"], a["Hkv"], a["D"], *a["qs"], a["k"], a["v"], a["ks"], a["vs"], a["pages"],
+        a["page_size"], a["table"], a["width"], a["lengths"], a["starts"], a["B"], a["window"], a["ahead"],
+        a["sinks"], a["scale"], 0, a["ws"], a["size"], a["out"], None, None)
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(q=None), -1), (dict(N=0), -1), (dict(B=0), -1), (dict(page_size=24), -2), (dict(D=80), -2),
+    (dict(ks=16), -1), (dict(table=None), -1), (dict(starts=None), -1), (dict(pages=0), -1), (dict(width=0), -1),
+    (dict(width=1 << 21), -1), (dict(qs=(255, 64)), -1), (dict(Hq=3), -1), (dict(scale=-1.0), -1),
+    (dict(width=60000), -1),  # (needs a workspace)
+])
+def test_paged_entry_point_rejects(bad, code):
+    assert _paged(**bad) == code
+
+
+def test_cache_entry_points_reject():
+    L = _lib.load()
+    ok = [16, 16, 2, 2, 64, 128, 64, 128, 64, 16, 16, None, None, 4, 16, 16, 3, 16, 16, 2, None, None]
+    for i, value, code in ((0, None, -1), (2, 0, -1), (4, 72, -2), (5, 127, -1), (11, 16, -1), (13, 0, -1),
+                           (14, 17, -2), (15, None, -1), (18, None, -1), (19, 0, -1)):
+        bad = list(ok)
+        bad[i] = value
+        assert L.solattn_cache_write(*bad) == code, i
+    ok = [16, 16, None, None, 4, 16, 16, 3, 16, 2, 2, 64, 5, 16, 16, None, None]
+    for i, value, code in ((0, None, -1), (2, 16, -1), (5, 5, -2), (12, 0, -1), (13, 8, -1), (11, 32, -2)):
+        bad = list(ok)
+        bad[i] = value
+        assert L.solattn_cache_read(*bad) == code, i
+
+
+def test_workspace_sizes():
+    """Short calls need none; long ones hold 16 rows of D + 2 floats per split."""
+    L = _lib.load()
+    assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 2, 64, 0, 0, 0) == 0
+    assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 3, 64, 0, 0, 0) == -1
+    size = L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 16, 0, 0, 0)
+    assert size > 0 and size % (16 * 130 * 4) == 0
+    # A window bounds what is split, however wide the table is.
+    assert L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 1 << 18, 64, 0, 4) == 0
