@@ -348,20 +348,22 @@ SOLATTN_API int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_
  * solattn_paged_attention: the packed queries q [N, Hq, D] (strides q_sT, q_sH) against their
  * sequences' keys under the visibility rule of solattn_window_attention with p = key_lengths[b] -
  * (new tokens of b) + i; out is a contiguous [N, Hq, D].  Rows behind the last sequence are left as
- * they are, or with zero_tail != 0 set to zero.  Workspace as above.
+ * they are, or with zero_tail != 0 set to zero.  most_new: the most new tokens that a sequence has,
+ * or 0 (not known); it only steers which kernels are launched, every result is right whatever it
+ * says.  Workspace as above.
  */
 SOLATTN_API int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
                       int64_t q_sT, int64_t q_sH, const void* k_pages, const void* v_pages,
                       const void* k_scale, const void* v_scale, int64_t pages, int64_t page_size,
                       const int32_t* page_table, int64_t table_width, const int32_t* key_lengths,
-                      const int32_t* query_starts, int64_t B, int64_t window, int64_t lookahead,
-                      int64_t sink_tokens, float scale, int zero_tail, void* workspace,
+                      const int32_t* query_starts, int64_t B, int64_t most_new, int64_t window,
+                      int64_t lookahead, int64_t sink_tokens, float scale, int zero_tail, void* workspace,
                       int64_t workspace_bytes, void* out, int32_t* status, void* stream);
 
 /* Workspace bytes of solattn_paged_attention, or -1 on an invalid shape. */
 SOLATTN_API int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                      int64_t page_size, int64_t table_width, int64_t window, int64_t lookahead,
-                      int64_t sink_tokens);
+                      int64_t page_size, int64_t table_width, int64_t most_new, int64_t window,
+                      int64_t lookahead, int64_t sink_tokens);
 
 /*
  * Writes the new tokens' K and V rows (packed BF16 [N, Hkv, D], strides k_sT ...) to their places in

@@ -44,11 +44,10 @@
 //              counts (built one item ahead), Q; then the K ring (slot refilled when S has
 //              completed) and the V ring (slot refilled when P V has completed), by TMA, or by
 //              gathering rows with cp.async for indexed inputs.
-#include <cudaTypedefs.h>
-
 #include <cstring>
 
 #include "sm100.cuh"
+#include "tensormap.cuh"
 
 namespace solattn {
 
@@ -1100,31 +1099,6 @@ cudaError_t launch_route(const AttnParams& p, int D, cudaStream_t stream);  // r
 
 namespace {
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  return fn;
-}
-
-// BF16 tensor map with 128-byte swizzle; dims/strides listed innermost first (strides in
-// bytes for dims 1..rank-1).
-bool make_map(CUtensorMap* map, const void* base, uint32_t rank, const cuuint64_t* dims,
-              const cuuint64_t* strides, const cuuint32_t* box) {
-  PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
-  if (!fn) return false;
-  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides,
-            box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // 4-D map over a BTHD view [B, T, H, D] with box {64, rows, 1, 1}.
 bool make_bthd_map(CUtensorMap* map, const TensorView& x, int B, int T, int H, int D,
                    uint32_t rows) {
@@ -1133,7 +1107,7 @@ bool make_bthd_map(CUtensorMap* map, const TensorView& x, int B, int T, int H, i
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B};
   const cuuint64_t strides[3] = {(cuuint64_t)x.sT * 2, (cuuint64_t)x.sH * 2, sb};
   const cuuint32_t box[4] = {64, rows, 1, 1};
-  return make_map(map, x.ptr, 4, dims, strides, box);
+  return make_bf16_map(map, x.ptr, 4, dims, strides, box);
 }
 
 // 4-D map over the pooled [B, H, nkb, D] statistics with box {64, 64, 1, 1}.
@@ -1142,7 +1116,7 @@ bool make_pooled_map(CUtensorMap* map, const __nv_bfloat16* base, int B, int H, 
   const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)nkb * D * 2,
                                  (cuuint64_t)H * nkb * D * 2};
   const cuuint32_t box[4] = {64, (cuuint32_t)kBlock, 1, 1};
-  return make_map(map, base, 4, dims, strides, box);
+  return make_bf16_map(map, base, 4, dims, strides, box);
 }
 
 template <int D>

@@ -1,0 +1,1008 @@
+// Attention of many query rows: a chunk of new tokens over a paged BF16 or E4M3 cache, or windowed
+// attention over contiguous K/V, on the tensor cores (tcgen05 with TMEM accumulators).
+//
+// Same mathematics as rows.cu: one pass over the keys with a running maximum, FP32 sums, P rounded to
+// BF16 for P V.  An item is 256 rows ((token, head) pairs of one sequence and K/V head, see paged.cuh),
+// two stages of 128 rows that share every K/V tile of 128 keys, and a share of the keys the rows need.
+// One persistent CTA per SM works through its items; the stages take turns on the tensor core, one
+// stage's softmax running while the other's products do:
+//
+//   S_0(i) S_1(i) | P_0(i) V  S_0(i+1) | P_1(i) V  S_1(i+1) | ...
+//
+// Warps: 0-3 and 4-7 softmax of stage 0 and 1 (a thread per row), 8 issues the MMAs, 9 loads K and V
+// (TMA; E4M3: bulk copies of codes and scales), 10 completes V tiles (rows behind the last key become
+// zeros), 11 finds the items and loads Q; E4M3 has 12-15 besides, which convert codes to BF16 tiles.
+// TMEM (512 columns): S_0, S_1 (128 columns each; P, as BF16 pairs, over the first 64), O_0, O_1.
+//
+// Keys that a row does not see have no influence whatever they hold: S is replaced by -inf.  Where V
+// is not finite, P = 0 times V would be NaN; an item whose result is not finite is therefore done
+// again at the end, carefully: warp 10 (or the converters) zeroes every V row that is not finite and
+// the softmax warps add what each row sees of it.
+#include <cstring>
+
+#include "join.cuh"
+#include "sm100.cuh"
+#include "tensormap.cuh"
+
+namespace solattn {
+
+namespace {
+
+using namespace sm100;
+
+constexpr int kStageRows = 128;
+constexpr int kItemRows = 256;  // two stages
+constexpr int kKeys = 128;      // keys of a tile
+constexpr int kSoftmaxWarps = 8;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kCheckWarp = 10, kItemWarp = 11, kConvWarp0 = 12;
+constexpr int kConvWarps = 4;
+constexpr int kBox = kKeys * 128;  // 128 rows x 64 BF16 columns, 128-byte swizzled
+constexpr uint32_t kTmemCols = 512, kTmemS = 0, kTmemO = 256;  // stage s at + 128 s
+constexpr int kRedoBits = 1024;
+
+template <int D, int KV>
+struct ChunkCfg {
+  static constexpr bool kCodes = KV == kPagedE4m3;
+  static constexpr int kThreads = kCodes ? 512 : 384;
+  // Registers: the launch's threads x registers divided between the softmax warpgroups and the rest
+  // (setmaxnreg); the host checks that the kernel was compiled to kLaunchRegs.
+  static constexpr int kLaunchRegs = kCodes ? 128 : 168;
+  static constexpr int kSoftmaxRegs = kCodes ? 184 : 208;
+  static constexpr int kOtherRegs = kCodes ? 72 : 88;
+  static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
+                "the register split must fit in what the launch holds");
+  static constexpr int kTile = kKeys * D * 2;  // a K, V or stage's Q tile
+  static constexpr int kQBufs = D == 64 ? 2 : 1;
+  static constexpr int kSlots = D == 64 ? 3 : 2;  // K slots = V slots
+  static constexpr int kCodeTile = kCodes ? kKeys * D : 0;
+  static constexpr int kCodeSlots = kCodes ? (D == 64 ? 4 : 2) : 0;
+  static constexpr int kQ = 0;
+  static constexpr int kK = kQBufs * 2 * kTile;
+  static constexpr int kV = kK + kSlots * kTile;
+  static constexpr int kCode = kV + kSlots * kTile;
+  static constexpr int kScale = kCode + kCodeSlots * kCodeTile;  // 128 scales per code slot
+  static constexpr int kBars = kScale + kCodeSlots * kKeys;
+  // Barriers.
+  static constexpr int ITEM_FULL = 0, ITEM_EMPTY = 2, Q_FULL = 4, Q_EMPTY = 6, S_FULL = 8, P_FULL = 10,
+                       PV_DONE = 12, O_FREE = 14, DRAIN = 16, K_FULL = 17, K_EMPTY = K_FULL + kSlots,
+                       V_FULL = K_EMPTY + kSlots, V_OK = V_FULL + kSlots, V_EMPTY = V_OK + kSlots,
+                       CODE_FULL = V_EMPTY + kSlots, CODE_EMPTY = CODE_FULL + kCodeSlots,
+                       NBARS = CODE_EMPTY + kCodeSlots;
+  static constexpr int kMisc = (kBars + NBARS * 8 + 15) & ~15;  // [0] TMEM address, [1] abort flag
+  static constexpr int kItems = kMisc + 16;                     // two item descriptions of 32 words
+  static constexpr int kBad = kItems + 2 * 128;                 // per V slot: bitmask of zeroed keys
+  static constexpr int kRedo = kBad + kSlots * 16;
+  static constexpr int kBytes = 1024 + kRedo + kRedoBits / 8;
+  static_assert(kBytes <= 227 * 1024, "shared memory of an SM");
+  static_assert(kSlots * 16 % 16 == 0 && kScale % 16 == 0, "bulk copies need 16-byte boundaries");
+};
+
+// An item as the item warp publishes it.
+struct Item {
+  int b;       // sequence, -1: no more items
+  int h;       // K/V head
+  int row0;    // first (token, head) row within the sequence
+  int rows;    // rows (1 .. 256)
+  int n, L, start;
+  int low, high;      // keys that some row sees: [low, high] and those below min(sinks, high + 1)
+  KeyTiles all;       // tiles of both stages
+  KeyTiles stage[2];  // tiles that each stage needs
+  int c0, c1;         // this split's part of all's list
+  int splits;         // of the item's row tile
+  int part;           // index of the partial result (splits > 1)
+  int redo;           // bit of the redo mask
+  int careful;
+};
+static_assert(sizeof(Item) <= 128, "item slot");
+
+// Whether no row of the item sees key `key`, and whether none sees any of [a, a + n).
+__device__ __forceinline__ bool unseen(const Item& it, int sinks, int key) {
+  return key > it.high || (key < it.low && key >= sinks);
+}
+__device__ __forceinline__ bool unseen(const Item& it, int sinks, int a, int n) {
+  return a > it.high || (a + n <= it.low && a >= sinks);
+}
+
+__device__ __forceinline__ bool needs(const KeyTiles& k, int t) { return t < k.sink || (t >= k.from && t < k.to); }
+
+// Bounded waits: on running out, the error is noted and the CTA's abort flag ends every role.
+struct Ctl {
+  volatile int* abort;
+  int32_t* status;
+};
+__device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, const Ctl& c) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (true) {
+    if (*c.abort) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    if (clock64() - t0 > kWaitLimitCycles) {
+      *c.abort = 1;
+      note(c.status, kStatusWaitTimeout);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool waitw(uint32_t bar, uint32_t parity, const Ctl& c) {
+  const bool ok = wait1(bar, parity, c);
+  return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void wait_quiet(uint32_t bar, uint32_t parity) {
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > kWaitLimitCycles) return;
+}
+
+// Loads issued into ring slot s of `slots` after `issued` loads in total.
+__device__ __forceinline__ int loads_into(int issued, int s, int slots) {
+  return issued > s ? (issued - s + slots - 1) / slots : 0;
+}
+
+template <int N>
+__device__ __forceinline__ void set_regs_more() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void set_regs_less() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+
+__device__ __forceinline__ void sts128(uint32_t a, const uint4& v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 lds128v(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(r) : "r"(taddr));
+  return r;
+}
+
+// Byte offset of the 16-byte piece c (of D / 8) of row r in a tile of 64-column boxes.
+__device__ __forceinline__ uint32_t tile_off(int r, int c) {
+  return (uint32_t)((c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// Columns [0, n) of a 32-column word of a tile, n clamped.
+__device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+// Finds item `i` of the launch.  Items run head by head (those in flight share K/V in the L2), within
+// a head from the last row tile to the first (under a causal rule the longest first).
+template <int D>
+__device__ __forceinline__ bool find_item(const SeqParams& p, int64_t i, int lane, Item& it) {
+  const int64_t per_head = (int64_t)p.slots * p.splits;
+  it.h = (int)(i / per_head);
+  const int r = (int)(i % per_head);
+  const int slot = p.slots - 1 - r / p.splits, split = r % p.splits;
+  const Seq sq = find_seq<kItemRows>(p, slot, lane);
+  it.b = sq.b;
+  if (sq.b < 0 || !p.takes(sq.n)) return false;
+  it.row0 = sq.tile * kItemRows;
+  it.rows = min(kItemRows, sq.n * p.G - it.row0);
+  it.n = sq.n;
+  it.L = sq.L;
+  it.start = sq.start;
+  const int off = sq.L - sq.n;
+  const int last = it.row0 + it.rows - 1;
+  it.low = key_low(p, off + it.row0 / p.G);
+  it.high = key_high(p, sq.L, off + last / p.G);
+  it.all = key_tiles<kKeys>(p, sq.L, off + it.row0 / p.G, off + last / p.G);
+  const int last0 = it.row0 + min(it.rows, kStageRows) - 1;
+  it.stage[0] = key_tiles<kKeys>(p, sq.L, off + it.row0 / p.G, off + last0 / p.G);
+  if (it.rows > kStageRows) {
+    it.stage[1] = key_tiles<kKeys>(p, sq.L, off + (it.row0 + kStageRows) / p.G, off + last / p.G);
+  } else {
+    it.stage[1].sink = it.stage[1].from = it.stage[1].to = 0;
+  }
+  const int total = it.all.count();
+  it.splits = max(1, min(p.splits, (total + p.unit - 1) / p.unit));
+  if (split >= it.splits) return false;
+  it.c0 = (int)((int64_t)total * split / it.splits);
+  it.c1 = (int)((int64_t)total * (split + 1) / it.splits);
+  it.part = (slot * p.Hkv + it.h) * p.splits + split;
+  return true;
+}
+
+}  // namespace
+
+template <int D, int KV>
+__global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
+    chunk_kernel(const SeqParams p, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV) {
+  using C = ChunkCfg<D, KV>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  const uint32_t bar0 = sbase + C::kBars;
+  auto bar = [bar0](int i) { return bar0 + 8u * (uint32_t)i; };
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + C::kMisc);
+  Item* items = reinterpret_cast<Item*>(smem + C::kItems);  // [2], 128 bytes apart
+  auto item_slot = [items](int j) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + 128 * j); };
+  volatile uint32_t* bad = reinterpret_cast<volatile uint32_t*>(smem + C::kBad);
+  uint32_t* redo = reinterpret_cast<uint32_t*>(smem + C::kRedo);
+  const Ctl ctl{reinterpret_cast<volatile int*>(misc + 1), p.status};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < C::NBARS; ++i) {
+      uint32_t count = 1;
+      if (i >= C::ITEM_EMPTY && i < C::ITEM_EMPTY + 2) count = 3 + kSoftmaxWarps + (C::kCodes ? kConvWarps - 1 : 0);
+      if (i >= C::Q_FULL && i < C::Q_FULL + 2) count = 32;
+      if ((i >= C::P_FULL && i < C::P_FULL + 2) || (i >= C::O_FREE && i < C::O_FREE + 2)) count = 4;
+      if (C::kCodes && ((i >= C::K_FULL && i < C::K_FULL + C::kSlots) || (i >= C::V_OK && i < C::V_OK + C::kSlots)))
+        count = kConvWarps;
+      if (i >= C::CODE_EMPTY) count = kConvWarps;
+      mbar_init(bar(i), count);
+    }
+    misc[1] = 0;
+    mbar_fence_init();
+  }
+  if (tid < kRedoBits / 32) redo[tid] = 0u;
+  if (warp == 0) {
+    tmem_alloc(smem_u32(misc), kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+  // Every role reads an item's description once it is full, and lets go of it when it has what it
+  // needs (the softmax warps after the item's results are out).
+  auto next_item = [&](int k, Item& it) {
+    if (!waitw(bar(C::ITEM_FULL + (k & 1)), (uint32_t)(k >> 1) & 1u, ctl)) return false;
+    it = *item_slot(k & 1);
+    return it.b >= 0;
+  };
+  auto release_item = [&](int k) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(C::ITEM_EMPTY + (k & 1)));
+  };
+
+  if (warp < kSoftmaxWarps) {
+    // ------------------------------------------------------------------ softmax
+    set_regs_more<C::kSoftmaxRegs>();
+    const int st = warp >> 2, quarter = warp & 3;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + kTmemS + 128u * st + lane_base;
+    const uint32_t tO = tmem + kTmemO + 128u * st + lane_base;
+    const float sl2 = p.scale_log2;
+    int g = 0;   // tiles of this CTA's earlier items (K/V ring position)
+    int ns = 0;  // tiles of this stage so far
+    {
+      uint32_t z[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) z[j] = 0u;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) tmem_st32(tO + 32 * c, z);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::O_FREE + st));
+    }
+    bool ok = true;
+    for (int k = 0; ok; ++k) {
+      Item it;
+      if (!next_item(k, it)) break;
+      const int off = it.L - it.n;
+      const int wrow = st * kStageRows + quarter * 32;  // first row of the warp within the item
+      const bool warp_rows = wrow < it.rows;
+      const int row = min(wrow + lane, it.rows - 1);
+      const int tok = (it.row0 + row) / p.G;
+      const int hi = key_high(p, it.L, off + tok), lo = key_low(p, off + tok);
+      // What all rows of the warp see, and what any of them does.
+      const int all_hi = __shfl_sync(0xffffffffu, hi, 0), all_lo = __shfl_sync(0xffffffffu, lo, 31);
+      const int any_hi = __shfl_sync(0xffffffffu, hi, 31), any_lo = __shfl_sync(0xffffffffu, lo, 0);
+      const KeyTiles mine = it.stage[st];
+      float m_run = -INFINITY, l_run = 0.f;
+      bool has = false;
+      for (int i = it.c0; i < it.c1; ++i) {
+        const int t = it.all.at(i);
+        if (!needs(mine, t)) continue;
+        const int kb = t * kKeys;
+        const bool first = !has;
+        has = true;
+        if (!waitw(bar(C::S_FULL + st), (uint32_t)ns & 1u, ctl)) {
+          ok = false;
+          break;
+        }
+        ++ns;
+        tc_fence_after();
+        const bool active = warp_rows && kb <= any_hi && (kb + kKeys > any_lo || kb < p.sinks);
+        if (!active) {  // nothing of the tile is seen by these rows
+          uint32_t z[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] = 0u;
+          tmem_st32(tS, z);
+          tmem_st32(tS + 32, z);
+        } else {
+          uint32_t sv[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + 32 * c, sv[c]);
+          tmem_wait_ld();
+          const bool full = kb + kKeys - 1 <= all_hi && (kb >= all_lo || kb + kKeys <= p.sinks);
+          if (!full) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t vis = below(hi + 1 - kb - 32 * c) &
+                                   (~below(lo - kb - 32 * c) | below(p.sinks - kb - 32 * c));
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((vis >> j) & 1u)) sv[c][j] = __float_as_uint(-INFINITY);
+            }
+          }
+          float mx[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const uint32_t* s = &sv[x >> 1][16 * (x & 1)];
+            float a = fmax3(__uint_as_float(s[0]), __uint_as_float(s[1]), __uint_as_float(s[2]));
+            float b = fmax3(__uint_as_float(s[3]), __uint_as_float(s[4]), __uint_as_float(s[5]));
+            a = fmax3(a, __uint_as_float(s[6]), __uint_as_float(s[7]));
+            b = fmax3(b, __uint_as_float(s[8]), __uint_as_float(s[9]));
+            a = fmax3(a, __uint_as_float(s[10]), __uint_as_float(s[11]));
+            b = fmax3(b, __uint_as_float(s[12]), __uint_as_float(s[13]));
+            mx[x] = fmax3(fmaxf(a, b), __uint_as_float(s[14]), __uint_as_float(s[15]));
+          }
+          const float m_tile =
+              fmax3(fmax3(mx[0], mx[1], mx[2]), fmax3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * sl2;
+          // The running maximum moves only when it grows by more than 8 (a factor 256), so that O is
+          // rarely rescaled; P stays at most 256.
+          bool need = false;
+          float alpha = 1.f;
+          if (m_run == -INFINITY) {
+            m_run = fmaxf(m_run, m_tile);
+          } else if (m_tile > m_run + 8.f) {
+            need = true;
+            alpha = fast_exp2(m_run - m_tile);
+            l_run *= alpha;
+            m_run = m_tile;
+          }
+          const float m_use = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t kmul = f2_pack(sl2, sl2), negm = f2_pack(-m_use, -m_use);
+          uint64_t acc[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[c][j]), __uint_as_float(sv[c][j + 1])), kmul, negm),
+                        x0, x1);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              acc[(j >> 1) & 3] = f2_add(acc[(j >> 1) & 3], f2_pack(p0, p1));
+              pk[j / 2] = pack_bf16(p0, p1);
+            }
+            tmem_st16(tS + 16 * c, pk);
+          }
+          float a0, a1;
+          f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a0, a1);
+          l_run += a0 + a1;
+          if (__any_sync(0xffffffffu, need)) {
+            // O may be touched once the stage's P V before this tile's has completed.
+            if (!first && !waitw(bar(C::PV_DONE + st), (uint32_t)ns & 1u, ctl)) {
+              tmem_wait_st();
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t a2 = f2_pack(alpha, alpha);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + 32 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                float y0, y1;
+                f2_unpack(f2_mul(f2_pack(__uint_as_float(o[j]), __uint_as_float(o[j + 1])), a2), y0, y1);
+                o[j] = __float_as_uint(y0);
+                o[j + 1] = __float_as_uint(y1);
+              }
+              tmem_st32(tO + 32 * c, o);
+            }
+          }
+        }
+        tmem_wait_st();
+        if (it.careful) {
+          // V rows that were zeroed for not being finite: add what this row sees of them.
+          const int gi = g + i - it.c0, slot = gi % C::kSlots;
+          if (!waitw(bar(C::V_OK + slot), (uint32_t)(gi / C::kSlots) & 1u, ctl) ||
+              (!first && !waitw(bar(C::PV_DONE + st), (uint32_t)ns & 1u, ctl))) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int key = 0; key < kKeys; ++key) {
+            if (!((bad[4 * slot + (key >> 5)] >> (key & 31)) & 1u)) continue;
+            const int pos = kb + key;
+            const uint32_t pair = tmem_ld1(tS + (uint32_t)(key >> 1));
+            tmem_wait_ld();
+            const float pv = __uint_as_float((key & 1) ? (pair & 0xffff0000u) : (pair << 16));
+            const bool see = pos <= hi && (pos >= lo || pos < p.sinks);
+            const uint8_t* src;
+            float f = 1.f;
+            if (KV == kStrided) {
+              src = p.v + ((int64_t)it.b * p.v_sB + (int64_t)pos * p.v_sT + (int64_t)it.h * p.v_sH) * 2;
+            } else {
+              const int page = page_of(p, it.b, pos);
+              const int64_t r = (((int64_t)page * p.Hkv + it.h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+              src = p.v + r * (KV == kPagedE4m3 ? D : 2 * D);
+              if (KV == kPagedE4m3) f = e8m0_value(p.v_scale[r]);
+            }
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int d = 16 * c + j;
+                const float x = KV == kPagedE4m3
+                                    ? e4m3_value(src[d]) * f
+                                    : __uint_as_float((uint32_t) reinterpret_cast<const uint16_t*>(src)[d] << 16);
+                if (see) o[j] = __float_as_uint(__uint_as_float(o[j]) + pv * x);
+              }
+              tmem_st16(tO + 16 * c, o);
+              tmem_wait_st();
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::P_FULL + st));
+      }
+      if (!ok) break;
+      g += it.c1 - it.c0;
+      // ---- the item's rows: O / l (or the partial O, m, l), then O = 0 for the next item
+      if (has && !waitw(bar(C::PV_DONE + st), (uint32_t)(ns - 1) & 1u, ctl)) break;
+      tc_fence_after();
+      const bool mine_row = wrow + lane < it.rows;
+      const bool any = hi >= 0 && (hi >= lo || p.sinks > 0);
+      const float inv = any ? 1.f / l_run : 0.f;
+      const bool partial = it.splits > 1;
+      const int64_t prow = (int64_t)it.part * kItemRows + wrow + lane;
+      __nv_bfloat16* dst = p.out + ((int64_t)(it.start + tok) * p.Hq + it.h * p.G + (it.row0 + row) % p.G) * D;
+      float check = l_run * 0.f;  // not zero where a value is not finite
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (has) {
+          tmem_ld32(tO + 32 * c, o);
+          tmem_wait_ld();
+        } else {  // (O holds zeros)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+        }
+        if (mine_row) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) check = fmaf(__uint_as_float(o[j]), 0.f, check);
+          if (partial) {
+            float4* d4 = reinterpret_cast<float4*>(p.part + prow * D + 32 * c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              d4[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
+                                  __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              w[j] = any ? pack_bf16(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv) : 0u;
+            uint4* d4 = reinterpret_cast<uint4*>(dst + 32 * c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d4[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+          }
+        }
+        if (has) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0u;
+          tmem_st32(tO + 32 * c, o);
+        }
+      }
+      if (has) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::O_FREE + st));
+      }
+      if (partial && mine_row) {
+        float2* ml = reinterpret_cast<float2*>(p.part + (int64_t)p.slots * p.Hkv * p.splits * kItemRows * D) + prow;
+        *ml = make_float2(m_run, l_run);
+      }
+      if (!it.careful && __any_sync(0xffffffffu, mine_row && check != 0.f) && lane == 0)
+        atomicOr(&redo[it.redo >> 5], 1u << (it.redo & 31));
+      release_item(k);
+    }
+  } else {
+    set_regs_less<C::kOtherRegs>();
+    if (warp == kMmaWarp) {
+      // ---------------------------------------------------------------- MMA issue
+      constexpr uint32_t idS = idesc_bf16(kStageRows, kKeys, false);
+      constexpr uint32_t idO = idesc_bf16(kStageRows, D, true);
+      const uint64_t dK = smem_desc_sw128(sbase + C::kK, 16, 1024);
+      const uint64_t dV = smem_desc_sw128(sbase + C::kV, kBox, 1024);
+      int g = 0;
+      int np[2] = {0, 0};  // tiles with P V issued, per stage
+      int nf[2] = {0, 0};  // items with such tiles, per stage
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        Item it;
+        if (!next_item(k, it)) break;
+        release_item(k);
+        const int qb = k % C::kQBufs;
+        if (!waitw(bar(C::Q_FULL + qb), (uint32_t)(k / C::kQBufs) & 1u, ctl)) break;
+        fence_proxy_async_smem();  // Q rows were written by cp.async
+        const uint64_t dQ = smem_desc_sw128(sbase + C::kQ + (uint32_t)(qb * 2 * C::kTile), 16, 1024);
+        auto issue_s = [&](int s, int gi) {
+          const uint64_t q = dQ + (uint64_t)((s * C::kTile) >> 4);
+          const uint64_t kd = dK + (uint64_t)(((gi % C::kSlots) * C::kTile) >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint64_t o = (uint64_t)(((kk >> 2) * kBox + (kk & 3) * 32) >> 4);
+              mma_ss(tmem + kTmemS + 128u * s, q + o, kd + o, idS, kk > 0 ? 1u : 0u);
+            }
+            mma_commit(bar(C::S_FULL + s));
+          }
+          __syncwarp();
+        };
+        const int count = it.c1 - it.c0;
+        // Q may be replaced once the item's last S is done.
+        auto release_q = [&]() {
+          if (elect_one()) mma_commit(bar(C::Q_EMPTY + qb));
+          __syncwarp();
+        };
+        if (count > 0) {
+          if (!waitw(bar(C::K_FULL + g % C::kSlots), (uint32_t)(g / C::kSlots) & 1u, ctl)) break;
+          tc_fence_after();
+          if (C::kCodes) fence_proxy_async_smem();
+          const int t = it.all.at(it.c0);
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
+            if (needs(it.stage[s], t)) issue_s(s, g);
+          if (elect_one()) mma_commit(bar(C::K_EMPTY + g % C::kSlots));
+          __syncwarp();
+        }
+        if (count <= 1) release_q();
+        bool started[2] = {false, false};
+        for (int i = 0; i < count; ++i) {
+          const int gi = g + i, sl = gi % C::kSlots;
+          const int t = it.all.at(it.c0 + i);
+          const bool more = i + 1 < count;
+          const int t1 = more ? it.all.at(it.c0 + i + 1) : 0;
+          if (!waitw(bar(C::V_OK + sl), (uint32_t)(gi / C::kSlots) & 1u, ctl) ||
+              (more && !waitw(bar(C::K_FULL + (gi + 1) % C::kSlots), (uint32_t)((gi + 1) / C::kSlots) & 1u, ctl))) {
+            ok = false;
+            break;
+          }
+          if (C::kCodes) fence_proxy_async_smem();
+          const uint64_t vd = dV + (uint64_t)((sl * C::kTile) >> 4);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (needs(it.stage[s], t)) {
+              // The stage's first tile of an item: O has been read and zeroed by the epilogue of the last
+              // item that used it (a stage without tiles in an item leaves the barrier alone, so that
+              // its softmax warps cannot run ahead of this warp's phases).
+              if (!started[s]) {
+                started[s] = true;
+                if (!waitw(bar(C::O_FREE + s), (uint32_t)nf[s] & 1u, ctl)) {
+                  ok = false;
+                  break;
+                }
+                ++nf[s];
+              }
+              if (!waitw(bar(C::P_FULL + s), (uint32_t)np[s] & 1u, ctl)) {
+                ok = false;
+                break;
+              }
+              ++np[s];
+              tc_fence_after();
+              if (elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kKeys / 16; ++kk)
+                  mma_ts(tmem + kTmemO + 128u * s, tmem + kTmemS + 128u * s + 8u * kk,
+                         vd + (uint64_t)((kk * 16 * 128) >> 4), idO, 1u);
+                mma_commit(bar(C::PV_DONE + s));
+              }
+              __syncwarp();
+            }
+            if (more && needs(it.stage[s], t1)) issue_s(s, gi + 1);
+          }
+          if (!ok) break;
+          if (elect_one()) {
+            mma_commit(bar(C::V_EMPTY + sl));
+            if (more) mma_commit(bar(C::K_EMPTY + (gi + 1) % C::kSlots));
+          }
+          __syncwarp();
+          if (i + 2 == count) release_q();
+        }
+        g += count;
+      }
+      if (lane == 0) {
+        mma_commit(bar(C::DRAIN));
+        wait_quiet(bar(C::DRAIN), 0);
+      }
+      __syncwarp();
+    } else if (warp == kLoadWarp) {
+      // ---------------------------------------------------------------- K and V loads
+      int g = 0;
+      int issued[2] = {0, 0};  // K and V loads
+      bool ok = true;
+      const int ps = 1 << p.page_shift;
+      for (int k = 0; ok; ++k) {
+        Item it;
+        if (!next_item(k, it)) break;
+        release_item(k);
+        const int count = it.c1 - it.c0;
+        // Lane l's page of tile i (piece l of the tile), fetched one tile ahead; -1: nobody sees it, so
+        // it is not loaded, whatever the page table says.
+        auto fetch = [&](int i) {
+          const int key = it.all.at(it.c0 + i) * kKeys + lane * ps;
+          if (KV == kStrided || lane * ps >= kKeys || unseen(it, p.sinks, key, ps)) return -1;
+          return page_of(p, it.b, key);
+        };
+        int page = count > 0 ? fetch(0) : -1;
+        for (int i = 0; i < count; ++i) {
+          const int gi = g + i, t = it.all.at(it.c0 + i), kb = t * kKeys;
+          const int next_page = i + 1 < count ? fetch(i + 1) : -1;
+          const int pieces = __popc(__ballot_sync(0xffffffffu, page >= 0));
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {  // K, then V
+            if constexpr (!C::kCodes) {
+              const int sl = gi % C::kSlots;
+              const int full = (z ? C::V_FULL : C::K_FULL) + sl, empty = (z ? C::V_EMPTY : C::K_EMPTY) + sl;
+              if (gi >= C::kSlots && !waitw(bar(empty), (uint32_t)(gi / C::kSlots - 1) & 1u, ctl)) {
+                ok = false;
+                break;
+              }
+              const uint32_t dst = sbase + (uint32_t)((z ? C::kV : C::kK) + sl * C::kTile);
+              const CUtensorMap* map = z ? &tmV : &tmK;
+              if constexpr (KV == kStrided) {
+                if (lane == 0) {
+                  mbar_expect_tx(bar(full), C::kTile);
+#pragma unroll
+                  for (int j = 0; j < D / 64; ++j) tma_load_4d(dst + j * kBox, map, bar(full), 64 * j, kb, it.h, it.b);
+                }
+              } else {
+                if (lane == 0) mbar_expect_tx(bar(full), (uint32_t)(pieces * ps * D * 2));
+                __syncwarp();
+                const int piece = lane / (D / 64), j = lane % (D / 64);
+                const int pg = __shfl_sync(0xffffffffu, page, piece);
+                if (piece * ps < kKeys && pg >= 0)
+                  tma_load_3d(dst + j * kBox + piece * ps * 128, map, bar(full), 64 * j, 0, pg * p.Hkv + it.h);
+              }
+            } else {
+              const int ci = 2 * gi + z, sl = ci % C::kCodeSlots;
+              if (ci >= C::kCodeSlots &&
+                  !waitw(bar(C::CODE_EMPTY + sl), (uint32_t)(ci / C::kCodeSlots - 1) & 1u, ctl)) {
+                ok = false;
+                break;
+              }
+              const uint32_t dst = sbase + (uint32_t)(C::kCode + sl * C::kCodeTile);
+              const uint32_t sdst = sbase + (uint32_t)(C::kScale + sl * kKeys);
+              if (lane == 0) mbar_expect_tx(bar(C::CODE_FULL + sl), (uint32_t)(pieces * ps * (D + 1)));
+              __syncwarp();
+              if (page >= 0) {
+                const int64_t row = ((int64_t)page * p.Hkv + it.h) << p.page_shift;
+                bulk_copy_g2s(dst + lane * ps * D, (z ? p.v : p.k) + row * D, ps * D, bar(C::CODE_FULL + sl));
+                bulk_copy_g2s(sdst + lane * ps, (z ? p.v_scale : p.k_scale) + row, ps, bar(C::CODE_FULL + sl));
+              }
+            }
+            ++issued[z];
+            __syncwarp();
+          }
+          if (!ok) break;
+          page = next_page;
+        }
+        g += count;
+      }
+      // After an abort no copy may land in shared memory of an exited CTA.
+      if (*ctl.abort && lane == 0) {
+        if constexpr (C::kCodes) {
+          for (int s = 0; s < C::kCodeSlots; ++s) {
+            const int n = loads_into(issued[0] + issued[1], s, C::kCodeSlots);
+            if (n) wait_quiet(bar(C::CODE_FULL + s), (uint32_t)(n - 1) & 1u);
+          }
+        } else {
+          for (int s = 0; s < C::kSlots; ++s) {
+            const int nk = loads_into(issued[0], s, C::kSlots), nv = loads_into(issued[1], s, C::kSlots);
+            if (nk) wait_quiet(bar(C::K_FULL + s), (uint32_t)(nk - 1) & 1u);
+            if (nv) wait_quiet(bar(C::V_FULL + s), (uint32_t)(nv - 1) & 1u);
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == kCheckWarp) {
+      // ---------------------------------------------------------------- V tiles of BF16 sources
+      if constexpr (!C::kCodes) {
+        int g = 0;
+        bool ok = true;
+        for (int k = 0; ok; ++k) {
+          Item it;
+          if (!next_item(k, it)) break;
+          release_item(k);
+          for (int i = it.c0; i < it.c1; ++i, ++g) {
+            const int sl = g % C::kSlots;
+            if (!waitw(bar(C::V_FULL + sl), (uint32_t)(g / C::kSlots) & 1u, ctl)) {
+              ok = false;
+              break;
+            }
+            const int kb = it.all.at(i) * kKeys;
+            const uint32_t sv = sbase + (uint32_t)(C::kV + sl * C::kTile);
+            // Rows that nobody sees (behind the last key, or beside the window) hold whatever the page or
+            // the slot held: zeros instead.
+            const bool edge = kb + kKeys - 1 > it.high || (kb < it.low && kb + kKeys > p.sinks);
+            if (edge || it.careful) {
+#pragma unroll 1
+              for (int j = 0; j < kKeys / 32; ++j) {
+                const int r = 32 * j + lane;
+                const bool behind = unseen(it, p.sinks, kb + r);
+                uint32_t acc = 0u;
+                if (it.careful && !behind) {
+#pragma unroll 1
+                  for (int c = 0; c < D / 8; ++c) {
+                    const uint4 v = lds128v(sv + tile_off(r, c));
+                    acc = bf16x2_fma(v.x, 0u, acc);
+                    acc = bf16x2_fma(v.y, 0u, acc);
+                    acc = bf16x2_fma(v.z, 0u, acc);
+                    acc = bf16x2_fma(v.w, 0u, acc);
+                  }
+                }
+                const bool wrong = (acc & 0x7fff7fffu) != 0u;
+                if (wrong || behind) {
+#pragma unroll 1
+                  for (int c = 0; c < D / 8; ++c) sts128(sv + tile_off(r, c), make_uint4(0, 0, 0, 0));
+                }
+                const uint32_t bits = __ballot_sync(0xffffffffu, wrong);
+                if (lane == 0) bad[4 * sl + j] = bits;
+              }
+              fence_proxy_async_smem();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::V_OK + sl));
+          }
+        }
+      }
+    } else if (warp == kItemWarp) {
+      // ---------------------------------------------------------------- items and Q
+      const int64_t total = (int64_t)p.slots * p.splits * p.Hkv;
+      const int64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
+      int shift = 0;  // redo bits cover 2^shift items when a CTA has more than kRedoBits
+      while ((per_cta >> shift) > kRedoBits - 1) ++shift;
+      int k = 0;
+      bool ok = true;
+      auto publish = [&](const Item& it) {
+        if (k >= 2 && !waitw(bar(C::ITEM_EMPTY + (k & 1)), (uint32_t)((k >> 1) - 1) & 1u, ctl)) return false;
+        if (lane == 0) {
+          *item_slot(k & 1) = it;
+          mbar_arrive(bar(C::ITEM_FULL + (k & 1)));
+        }
+        __syncwarp();
+        return true;
+      };
+#pragma unroll 1
+      for (int pass = 0; pass < 2 && ok; ++pass) {
+        if (pass == 1) {
+          // Every item published so far is finished (its softmax warps let go of it at their end).
+          for (int j = max(0, k - 2); j < k && ok; ++j)
+            ok = waitw(bar(C::ITEM_EMPTY + (j & 1)), (uint32_t)(j >> 1) & 1u, ctl);
+          if (!ok) break;
+        }
+        int64_t ord = 0;
+#pragma unroll 1
+        for (int64_t i = blockIdx.x; i < total && ok; i += gridDim.x, ++ord) {
+          const int bit = (int)(ord >> shift);
+          if (pass == 1 && !((*reinterpret_cast<volatile uint32_t*>(&redo[bit >> 5]) >> (bit & 31)) & 1u)) continue;
+          Item it;
+          if (!find_item<D>(p, i, lane, it)) continue;
+          it.redo = bit;
+          it.careful = pass;
+          if (!publish(it)) {
+            ok = false;
+            break;
+          }
+          const int qb = k % C::kQBufs;
+          if (k >= C::kQBufs && !waitw(bar(C::Q_EMPTY + qb), (uint32_t)(k / C::kQBufs - 1) & 1u, ctl)) {
+            ok = false;
+            break;
+          }
+          // Q: D / 8 lanes copy a row; lane l holds the offsets of rows l, l + 32, ...
+          const __nv_bfloat16* base = p.q + (p.table ? (int64_t)it.start * p.q_sT : (int64_t)it.b * p.q_sB) +
+                                      (int64_t)it.h * p.G * p.q_sH;
+          const uint32_t sq = sbase + (uint32_t)(C::kQ + qb * 2 * C::kTile);
+          constexpr int kPer = 32 / (D / 8);  // rows of a warp instruction
+          const int c = lane % (D / 8);
+#pragma unroll 1
+          for (int j = 0; j < kItemRows / 32; ++j) {
+            const int r = it.row0 + min(32 * j + lane, it.rows - 1);
+            const int64_t mo = (int64_t)(r / p.G) * p.q_sT + (int64_t)(r % p.G) * p.q_sH;
+#pragma unroll
+            for (int x = 0; x < 32 / kPer; ++x) {
+              const int rr = x * kPer + lane / (D / 8);
+              const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
+              const int row = 32 * j + rr;
+              cp_async16(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
+                         base + o + 8 * c, row < it.rows ? 16 : 0);
+            }
+          }
+          cp_async_mbar_arrive_noinc(bar(C::Q_FULL + qb));
+          ++k;
+        }
+      }
+      cp_async_wait_all();
+      if (ok) {
+        Item end;
+        end.b = -1;
+        publish(end);
+      }
+      if (p.zero_tail) zero_tail<D>(p, blockIdx.x, gridDim.x, lane, 32);
+    } else if constexpr (C::kCodes) {
+      // ---------------------------------------------------------------- E4M3 codes to BF16 tiles
+      const int ct = tid - kConvWarp0 * 32;
+      constexpr int kPieces = D / 16;  // 16-code pieces of a row
+      int g = 0;
+      bool ok = true;
+      for (int k = 0; ok; ++k) {
+        Item it;
+        if (!next_item(k, it)) break;
+        release_item(k);
+        for (int i = it.c0; i < it.c1 && ok; ++i, ++g) {
+          const int kb = it.all.at(i) * kKeys, sl = g % C::kSlots;
+#pragma unroll 1
+          for (int z = 0; z < 2; ++z) {
+            const int ci = 2 * g + z, cs = ci % C::kCodeSlots;
+            if (!waitw(bar(C::CODE_FULL + cs), (uint32_t)(ci / C::kCodeSlots) & 1u, ctl) ||
+                (g >= C::kSlots &&
+                 !waitw(bar((z ? C::V_EMPTY : C::K_EMPTY) + sl), (uint32_t)(g / C::kSlots - 1) & 1u, ctl))) {
+              ok = false;
+              break;
+            }
+            const uint32_t src = sbase + (uint32_t)(C::kCode + cs * C::kCodeTile);
+            const uint8_t* sc = smem + C::kScale + cs * kKeys;
+            const uint32_t dst = sbase + (uint32_t)((z ? C::kV : C::kK) + sl * C::kTile);
+#pragma unroll 2
+            for (int x = 0; x < kKeys * kPieces / 128; ++x) {
+              const int q = x * 128 + ct, r = q / kPieces, c = q % kPieces;
+              const bool behind = unseen(it, p.sinks, kb + r);
+              const uint4 w4 = lds128v(src + (uint32_t)(r * D + 16 * c));
+              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+              const uint32_t e = behind ? 0u : sc[r];
+              uint32_t y[8];
+              // value = code fields * 2^120 * 2^(e - 127): one factor where it is a BF16.
+              uint32_t f = e == 255u ? 0x7fc0u : e <= 134u ? (e + 120u) << 7 : 0x7f00u;
+              f |= f << 16;
+              uint32_t nan = 0u;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                nan |= e4m3_nan_bytes(w[j]);
+                y[2 * j] = bf16x2_mul(e4m3_fields(__byte_perm(w[j], 0u, 0x1404)), f);
+                y[2 * j + 1] = bf16x2_mul(e4m3_fields(__byte_perm(w[j], 0u, 0x3424)), f);
+              }
+              if (e > 134u && e < 255u) {
+                uint32_t f2 = (e - 7u) << 7;
+                f2 |= f2 << 16;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = bf16x2_mul(y[j], f2);
+              }
+              if (nan) {  // (rare) NaN codes: element by element
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const uint32_t two = w[j >> 1] >> (16 * (j & 1));
+                  if ((two & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
+                  if ((two & 0x7f00u) == 0x7f00u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
+                }
+              }
+              if (behind) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = 0u;
+              }
+              if (z && it.careful) {  // a row's pieces lie in one warp: all of it becomes zero
+                uint32_t acc = 0u;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc = bf16x2_fma(y[j], 0u, acc);
+                const uint32_t wrong = __ballot_sync(0xffffffffu, (acc & 0x7fff7fffu) != 0u);
+                const bool row_wrong = ((wrong >> (lane & ~(kPieces - 1))) & ((1u << kPieces) - 1u)) != 0u;
+                uint32_t* word = const_cast<uint32_t*>(&bad[4 * sl + (r >> 5)]);
+                if (c == 0) {
+                  if (row_wrong) atomicOr(word, 1u << (r & 31));
+                  else atomicAnd(word, ~(1u << (r & 31)));
+                }
+                if (row_wrong) {
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) y[j] = 0u;
+                }
+              }
+              sts128(dst + tile_off(r, 2 * c), make_uint4(y[0], y[1], y[2], y[3]));
+              sts128(dst + tile_off(r, 2 * c + 1), make_uint4(y[4], y[5], y[6], y[7]));
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              mbar_arrive(bar((z ? C::V_OK : C::K_FULL) + sl));
+              mbar_arrive(bar(C::CODE_EMPTY + cs));
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+namespace {
+
+// BF16 map over a contiguous source [B, T, H, D], box {64, 128, 1, 1}.
+bool strided_map(CUtensorMap* map, const uint8_t* x, int64_t sB, int64_t sT, int64_t sH, const SeqParams& p, int D) {
+  cuuint64_t sb = (cuuint64_t)sB * 2;
+  if (p.B == 1) sb = ((cuuint64_t)sT * 2 * (cuuint64_t)p.Tk + 15) & ~cuuint64_t(15);
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)p.Tk, (cuuint64_t)p.Hkv, (cuuint64_t)p.B};
+  const cuuint64_t strides[3] = {(cuuint64_t)sT * 2, (cuuint64_t)sH * 2, sb};
+  const cuuint32_t box[4] = {64, (cuuint32_t)kKeys, 1, 1};
+  return make_bf16_map(map, x, 4, dims, strides, box);
+}
+// BF16 map over pages [pages * Hkv, page_size, D], box {64, page_size, 1}.
+bool paged_map(CUtensorMap* map, const uint8_t* x, const SeqParams& p, int D) {
+  const cuuint64_t ps = cuuint64_t(1) << p.page_shift;
+  const cuuint64_t dims[3] = {(cuuint64_t)D, ps, (cuuint64_t)p.pages * p.Hkv};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, ps * D * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)ps, 1};
+  return make_bf16_map(map, x, 3, dims, strides, box);
+}
+
+template <int D, int KV>
+cudaError_t launch_chunk_kv(const SeqParams& p, cudaStream_t stream) {
+  using C = ChunkCfg<D, KV>;
+  CUtensorMap tmK, tmV;
+  memset(&tmK, 0, sizeof(tmK));
+  memset(&tmV, 0, sizeof(tmV));
+  if (KV == kStrided && (!strided_map(&tmK, p.k, p.k_sB, p.k_sT, p.k_sH, p, D) ||
+                         !strided_map(&tmV, p.v, p.v_sB, p.v_sT, p.v_sH, p, D)))
+    return cudaErrorInvalidValue;
+  if (KV == kPagedBf16 && (!paged_map(&tmK, p.k, p, D) || !paged_map(&tmV, p.v, p, D))) return cudaErrorInvalidValue;
+  auto* kernel = chunk_kernel<D, KV>;
+  // setmaxnreg divides exactly the registers that the launch holds: with fewer it would wait for good.
+  cudaFuncAttributes attr;
+  cudaError_t err = cudaFuncGetAttributes(&attr, kernel);
+  if (err != cudaSuccess) return err;
+  if (attr.numRegs != C::kLaunchRegs) return cudaErrorInvalidDeviceFunction;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+  if (err != cudaSuccess) return err;
+  int dev = 0, sms = 0;
+  err = cudaGetDevice(&dev);
+  if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (err != cudaSuccess) return err;
+  const int64_t items = (int64_t)p.slots * p.Hkv * p.splits;
+  kernel<<<(unsigned)(items < sms ? items : sms), C::kThreads, C::kBytes, stream>>>(p, tmK, tmV);
+  err = cudaGetLastError();
+  if (err != cudaSuccess || p.splits == 1) return err;
+  join_kernel<D, kItemRows, kKeys><<<dim3((unsigned)((int64_t)p.slots * p.Hkv), kItemRows / 16), kJoinThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_chunk(const SeqParams& p, int D, int kv, cudaStream_t stream) {
+  if (D == 128) {
+    if (kv == kStrided) return launch_chunk_kv<128, kStrided>(p, stream);
+    if (kv == kPagedBf16) return launch_chunk_kv<128, kPagedBf16>(p, stream);
+    return launch_chunk_kv<128, kPagedE4m3>(p, stream);
+  }
+  if (kv == kStrided) return launch_chunk_kv<64, kStrided>(p, stream);
+  if (kv == kPagedBf16) return launch_chunk_kv<64, kPagedBf16>(p, stream);
+  return launch_chunk_kv<64, kPagedE4m3>(p, stream);
+}
+
+}  // namespace solattn

@@ -1,0 +1,58 @@
+// Joins the splits of the attention kernels' rows.
+#pragma once
+
+#include "paged.cuh"
+
+namespace solattn {
+
+constexpr int kJoinThreads = 128;
+
+// out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - max m), over a row's partial results: O at
+// part[unit][R][D], m and l behind all of them.  R rows of a tile, T keys of a key tile, as in the
+// kernel that wrote them.  A CTA takes 16 rows of a tile, a warp one row at a time; the order over
+// the splits is fixed, so that a call gives the same bits each time.
+template <int D, int R, int T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = (int)(blockIdx.x % p.Hkv), slot = (int)(blockIdx.x / p.Hkv);
+  const Seq sq = find_seq<R>(p, slot, lane);
+  if (sq.b < 0 || !p.takes(sq.n)) return;
+  const int r_base = sq.tile * R, off = sq.L - sq.n;
+  const int rows = min(R, sq.n * p.G - r_base);
+  const KeyTiles kt = key_tiles<T>(p, sq.L, off + r_base / p.G, off + (r_base + rows - 1) / p.G);
+  const int ns = max(1, min(p.splits, (kt.count() + p.unit - 1) / p.unit));
+  if (ns == 1) return;
+  const int64_t unit0 = ((int64_t)slot * p.Hkv + h) * p.splits;
+  const float2* ml0 = reinterpret_cast<const float2*>(p.part + (int64_t)p.slots * p.Hkv * p.splits * R * D);
+  constexpr int kPer = D / 32;  // dims of a lane
+  const int r0 = 16 * blockIdx.y, r1 = min(rows, r0 + 16);
+  for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {
+    float mx = -INFINITY;
+    for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml0[(unit0 + s) * R + r].x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f, a[kPer];
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) a[x] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < ns; ++s) {
+      const float2 ml = ml0[(unit0 + s) * R + r];
+      const float f = fast_exp2(ml.x - base);
+      sum += ml.y * f;
+      const float* src = p.part + ((unit0 + s) * R + r) * D + kPer * lane;
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) a[x] += src[x] * f;
+    }
+    const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
+    const int high = key_high(p, sq.L, pos);
+    const bool any = high >= 0 && (high >= key_low(p, pos) || p.sinks > 0);
+    const float inv = any ? 1.f / sum : 0.f;
+    __nv_bfloat16* dst = p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + kPer * lane;
+#pragma unroll
+    for (int x = 0; x < kPer; x += 2)
+      *reinterpret_cast<uint32_t*>(dst + x) = any ? pack_bf16(a[x] * inv, a[x + 1] * inv) : 0u;
+  }
+}
+
+}  // namespace solattn

@@ -42,7 +42,9 @@ struct SeqParams {
   int window, ahead, sinks;
   int slots, splits, unit;  // row tiles over all sequences; splits of a tile; keys tiles per split
   int zero_tail;            // write zeros to the rows behind the last sequence
+  int min_new, max_new;     // new tokens of the sequences that this launch takes
   float scale_log2;         // softmax scale * log2(e)
+  __device__ __forceinline__ bool takes(int n) const { return n >= min_new && n <= max_new; }
 };
 
 struct CacheParams {
@@ -172,17 +174,17 @@ __device__ __forceinline__ int page_of(const SeqParams& p, int b, int key) {
   return page;
 }
 
-// Rows behind the last sequence of a packed call: zeros, when the caller asked for them.  Called by
-// all threads of the CTAs `part` of `parts`.
+// Rows behind the last sequence of a packed call become zeros: the share `part` of `parts`, by
+// `threads` threads.
 template <int D>
-__device__ __forceinline__ void zero_tail(const SeqParams& p, int part, int parts) {
-  if (!p.zero_tail || !p.table) return;
+__device__ __forceinline__ void zero_tail(const SeqParams& p, int part, int parts, int thread, int threads) {
+  if (!p.table) return;
   const int end = __ldg(p.starts + p.B);
   if (end < 0 || end >= p.N) return;
   const int64_t chunks = (int64_t)p.Hq * D / 8;  // 16-byte pieces of a token
   for (int64_t t = (int64_t)end + part; t < p.N; t += parts) {
     uint4* dst = reinterpret_cast<uint4*>(p.out + t * p.Hq * D);
-    for (int64_t i = threadIdx.x; i < chunks; i += blockDim.x) dst[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = thread; i < chunks; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
   }
 }
 

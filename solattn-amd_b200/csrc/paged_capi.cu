@@ -7,6 +7,7 @@
 
 namespace solattn {
 
+cudaError_t launch_chunk(const SeqParams& p, int D, int kv, cudaStream_t stream);
 cudaError_t launch_rows(const SeqParams& p, int D, int kv, cudaStream_t stream);
 cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream);
 cudaError_t launch_cache_read(const CacheParams& p, int D, cudaStream_t stream);
@@ -63,8 +64,62 @@ Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int6
   s.splits = cdiv(chunks, unit);
   return s;
 }
-int64_t split_bytes(const Split& s, int64_t Hkv, int64_t D) {
-  return s.splits > 1 ? s.slots * Hkv * s.splits * 16 * (D + 2) * 4 : 0;
+
+// How the chunk kernel divides a call: tiles of 256 rows and key splits of at least `unit` 128-key
+// tiles.  Its CTAs work through equal shares of the items, so the time is about (items per SM, rounded
+// up) * (tiles per item + 3), in key tiles; 3 is what starting and ending an item costs, and a join
+// about 4.  The split with the least such time is taken (the lengths being known only as bounds).
+Split chunk_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t cap, bool paged,
+                  const Rule& r) {
+  Split s;
+  const int64_t G = Hq / Hkv;
+  s.slots = paged ? N * G / 256 + B : B * cdiv(Tq * G, 256);
+  int64_t keys = cap;
+  if (r.window > 0 && r.lookahead >= 0) {
+    const int64_t span = r.window + r.lookahead + r.sinks + 256 / G + 1;
+    if (span < keys) keys = span;
+  }
+  const int64_t tiles = cdiv(keys, 128) + 1;
+  const int64_t items = Hkv * (paged ? cdiv(N * G, 256) + B / 2 : s.slots);
+  int64_t best = 0;
+  s.splits = 1;
+  for (int64_t n = 1; n <= 64 && n <= tiles; ++n) {
+    const int64_t time = cdiv(items * n, kSms) * (cdiv(tiles, n) + 3) + (n > 1 ? 4 : 0);
+    if (n == 1 || time < best) {
+      best = time;
+      s.splits = n;
+    }
+  }
+  s.unit = cdiv(tiles, s.splits);
+  return s;
+}
+
+int64_t split_bytes(const Split& s, int64_t tile_rows, int64_t Hkv, int64_t D) {
+  return s.splits > 1 ? s.slots * Hkv * s.splits * tile_rows * (D + 2) * 4 : 0;
+}
+
+// Which kernels a call takes.  The few-rows kernel reads its keys once per 16 rows, the chunk kernel
+// once per 256 but with tiles that are mostly empty for few rows; they meet at about kManyRows rows
+// of a sequence.  A packed call whose sequences may lie on both sides launches both, each for its own.
+constexpr int64_t kManyRows = 64;
+struct Choice {
+  bool few, many;
+  Split rows, chunk;
+  int64_t rows_bytes, chunk_bytes;
+};
+Choice choose(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most_new, int64_t cap,
+              bool paged, const Rule& r) {
+  Choice c;
+  const int64_t G = Hq / Hkv;
+  const int64_t most = paged ? (most_new > 0 && most_new < N ? most_new : N) * G : Tq * G;
+  const int64_t mean = paged ? N * G / B : Tq * G;
+  c.many = most >= kManyRows;
+  c.few = mean < kManyRows;
+  c.rows = rows_split(N, B, Hq, Hkv, Tq, cap, paged, r);
+  c.chunk = chunk_split(N, B, Hq, Hkv, Tq, cap, paged, r);
+  c.rows_bytes = c.few ? split_bytes(c.rows, 16, Hkv, D) : 0;
+  c.chunk_bytes = c.many ? split_bytes(c.chunk, 256, Hkv, D) : 0;
+  return c;
 }
 
 int check_heads(int64_t Hq, int64_t Hkv, int64_t D) {
@@ -98,16 +153,30 @@ void set_rule(SeqParams& p, const Rule& r, float scale) {
   p.scale_log2 = scale * 1.4426950408889634f;
 }
 
-int run(SeqParams& p, int64_t D, int kv, const Split& s, void* workspace, int64_t workspace_bytes,
+int run(SeqParams& p, int64_t D, int kv, const Choice& c, void* workspace, int64_t workspace_bytes,
         void* stream) {
-  if (s.slots * p.Hkv * s.splits >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
-  if (split_bytes(s, p.Hkv, D) > workspace_bytes) return SOLATTN_ERR_ARG;
-  if (s.splits > 1 && (!workspace || !aligned16(workspace))) return SOLATTN_ERR_ARG;
-  p.slots = (int)s.slots;
-  p.splits = (int)s.splits;
-  p.unit = (int)s.unit;
-  p.part = static_cast<float*>(workspace);
-  return from_cuda(launch_rows(p, (int)D, kv, static_cast<cudaStream_t>(stream)));
+  const int64_t need = c.rows_bytes + c.chunk_bytes;
+  if (c.few && c.rows.slots * p.Hkv * c.rows.splits >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  if (c.many && c.chunk.slots * p.Hkv * c.chunk.splits >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  if (need > workspace_bytes || (need > 0 && (!workspace || !aligned16(workspace)))) return SOLATTN_ERR_ARG;
+  // A sequence with n new tokens is the chunk kernel's iff n * G >= kManyRows, where both run.
+  const int64_t least = cdiv(kManyRows, p.G);
+  for (int many = 0; many < 2; ++many) {
+    if (!(many ? c.many : c.few)) continue;
+    SeqParams x = p;
+    const Split& s = many ? c.chunk : c.rows;
+    x.slots = (int)s.slots;
+    x.splits = (int)s.splits;
+    x.unit = (int)s.unit;
+    x.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (many ? c.rows_bytes : 0));
+    x.min_new = many && c.few ? (int)least : 0;
+    x.max_new = !many && c.many ? (int)least - 1 : 0x7fffffff;
+    x.zero_tail = p.zero_tail && !(many && c.few);
+    const int rc = from_cuda(many ? launch_chunk(x, (int)D, kv, static_cast<cudaStream_t>(stream))
+                                  : launch_rows(x, (int)D, kv, static_cast<cudaStream_t>(stream)));
+    if (rc) return rc;
+  }
+  return SOLATTN_OK;
 }
 
 int cache_params(CacheParams& p, const void* k_pages, const void* v_pages, const void* k_scale,
@@ -143,7 +212,8 @@ int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_
                                        int64_t D, int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_window(B, Tq, Tk, Hq, Hkv, D, r)) return -1;
-  return split_bytes(rows_split(B * Tq, B, Hq, Hkv, Tq, Tk, false, r), Hkv, D);
+  const Choice c = choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r);
+  return c.rows_bytes + c.chunk_bytes;
 }
 
 int solattn_window_attention(const void* q, const void* k, const void* v, int64_t B, int64_t Tq, int64_t Tk,
@@ -178,30 +248,30 @@ int solattn_window_attention(const void* q, const void* k, const void* v, int64_
   p.Tq = (int)Tq;
   p.Tk = (int)Tk;
   set_rule(p, r, scale);
-  return run(p, D, kStrided, rows_split(B * Tq, B, Hq, Hkv, Tq, Tk, false, r), workspace, workspace_bytes,
-             stream);
+  return run(p, D, kStrided, choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r), workspace, workspace_bytes, stream);
 }
 
 int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                                      int64_t page_size, int64_t table_width, int64_t window,
-                                      int64_t lookahead, int64_t sink_tokens) {
+                                      int64_t page_size, int64_t table_width, int64_t most_new,
+                                      int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_paged(N, B, Hq, Hkv, D, page_size, table_width, r)) return -1;
-  return split_bytes(rows_split(N, B, Hq, Hkv, 0, table_width * page_size, true, r), Hkv, D);
+  const Choice c = choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r);
+  return c.rows_bytes + c.chunk_bytes;
 }
 
 int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t q_sT,
                             int64_t q_sH, const void* k_pages, const void* v_pages, const void* k_scale,
                             const void* v_scale, int64_t pages, int64_t page_size, const int32_t* page_table,
                             int64_t table_width, const int32_t* key_lengths, const int32_t* query_starts,
-                            int64_t B, int64_t window, int64_t lookahead, int64_t sink_tokens, float scale,
-                            int zero_tail, void* workspace, int64_t workspace_bytes, void* out,
+                            int64_t B, int64_t most_new, int64_t window, int64_t lookahead,
+                            int64_t sink_tokens, float scale, int zero_tail, void* workspace, int64_t workspace_bytes, void* out,
                             int32_t* status, void* stream) {
   const Rule r{window, lookahead, sink_tokens};
   const int rc = check_paged(N, B, Hq, Hkv, D, page_size, table_width, r);
   if (rc) return rc;
   if (!q || !k_pages || !v_pages || !page_table || !key_lengths || !query_starts || !out ||
-      (k_scale == nullptr) != (v_scale == nullptr) || pages <= 0 || pages > 0x7fffffff)
+      (k_scale == nullptr) != (v_scale == nullptr) || pages <= 0 || pages * Hkv > 0x7fffffff || most_new < 0)
     return SOLATTN_ERR_ARG;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       (k_scale && (!aligned16(k_scale) || !aligned16(v_scale))) || !stride_ok(q_sT) || !stride_ok(q_sH))
@@ -231,7 +301,7 @@ int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, i
   p.zero_tail = zero_tail;
   set_rule(p, r, scale);
   return run(p, D, k_scale ? kPagedE4m3 : kPagedBf16,
-             rows_split(N, B, Hq, Hkv, 0, table_width * page_size, true, r), workspace, workspace_bytes,
+             choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r), workspace, workspace_bytes,
              stream);
 }
 

@@ -14,7 +14,7 @@
 // Keys that a row does not see have no influence whatever they hold: S is replaced by -inf, and a
 // chunk with a non-finite V (where P = 0 times V would be NaN) goes through exact_pv, which adds
 // only what each row sees.
-#include "paged.cuh"
+#include "join.cuh"
 
 namespace solattn {
 
@@ -138,9 +138,9 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
   const int split = (int)(blockIdx.x % p.splits);
   const int h = (int)((blockIdx.x / p.splits) % p.Hkv);
   const int slot = (int)(blockIdx.x / ((unsigned)p.splits * p.Hkv));
-  if (split == 0 && h == 0) zero_tail<D>(p, slot, p.slots);
+  if (split == 0 && h == 0 && p.zero_tail) zero_tail<D>(p, slot, p.slots, tid, kRowThreads);
   const Seq sq = find_seq<kTileRows>(p, slot, lane);
-  if (sq.b < 0) return;
+  if (sq.b < 0 || !p.takes(sq.n)) return;
   const int rows = min(kTileRows, sq.n * p.G - sq.tile * kTileRows);
   const int r_base = sq.tile * kTileRows;  // first (token, head) row of the tile
   const int off = sq.L - sq.n;             // position of token 0
@@ -472,51 +472,6 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
   }
 }
 
-// Joins the splits of a row: out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - max m).  One warp
-// takes a row; the order over the splits is fixed.
-template <int D>
-__global__ void __launch_bounds__(kRowThreads) rows_join_kernel(const SeqParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = (int)(blockIdx.x % p.Hkv), slot = (int)(blockIdx.x / p.Hkv);
-  const Seq sq = find_seq<kTileRows>(p, slot, lane);
-  if (sq.b < 0) return;
-  const int rows = min(kTileRows, sq.n * p.G - sq.tile * kTileRows);
-  const int r_base = sq.tile * kTileRows, off = sq.L - sq.n;
-  const KeyTiles kt =
-      key_tiles<kChunk>(p, sq.L, off + r_base / p.G, off + (r_base + rows - 1) / p.G);
-  const int ns = max(1, min(p.splits, (kt.count() + p.unit - 1) / p.unit));
-  if (ns == 1) return;
-  const int64_t unit0 = ((int64_t)slot * p.Hkv + h) * p.splits;
-  const float* ml0 = p.part + (int64_t)p.slots * p.Hkv * p.splits * kTileRows * D;
-  constexpr int kPer = D / 32;  // dims of a lane
-  for (int r = warp; r < rows; r += kWarps) {
-    float mx = -INFINITY;
-    for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml0[((unit0 + s) * kTileRows + r) * 2]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, a[kPer];
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) a[x] = 0.f;
-    for (int s = 0; s < ns; ++s) {
-      const float2 ml = *reinterpret_cast<const float2*>(ml0 + ((unit0 + s) * kTileRows + r) * 2);
-      const float f = fast_exp2(ml.x - base);
-      sum += ml.y * f;
-      const float* src = p.part + ((unit0 + s) * kTileRows + r) * D + kPer * lane;
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) a[x] += src[x] * f;
-    }
-    const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
-    const int high = key_high(p, sq.L, pos);
-    const bool any = high >= 0 && (high >= key_low(p, pos) || p.sinks > 0);
-    const float inv = any ? 1.f / sum : 0.f;
-    __nv_bfloat16* dst = p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + kPer * lane;
-#pragma unroll
-    for (int x = 0; x < kPer; x += 2)
-      *reinterpret_cast<uint32_t*>(dst + x) = any ? pack_bf16(a[x] * inv, a[x + 1] * inv) : 0u;
-  }
-}
-
 namespace {
 
 template <int D, int KV>
@@ -529,7 +484,7 @@ cudaError_t launch_rows_kv(const SeqParams& p, cudaStream_t stream) {
   rows_kernel<D, KV><<<(unsigned)ctas, kRowThreads, smem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1) return err;
-  rows_join_kernel<D><<<(unsigned)((int64_t)p.slots * p.Hkv), kRowThreads, 0, stream>>>(p);
+  join_kernel<D, kTileRows, kChunk><<<(unsigned)((int64_t)p.slots * p.Hkv), kJoinThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 

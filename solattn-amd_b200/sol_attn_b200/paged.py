@@ -106,11 +106,14 @@ class PagedPlan:
     ``query_starts[b + 1] - 1`` of the packed tensors and the sequence's last.  Page table entries
     of pages that no visible key needs may hold anything (a page given back, -1).  The tensors may
     be changed in place between calls (a captured graph reads their contents at each replay).
+    ``most_new``: the most new tokens of a sequence, where known; it helps to choose the kernels, and
+    results are right whatever it says.
     """
 
     page_table: torch.Tensor
     key_lengths: torch.Tensor
     query_starts: torch.Tensor
+    most_new: int = 0
 
     def __post_init__(self):
         t, n, s = self.page_table, self.key_lengths, self.query_starts
@@ -118,6 +121,7 @@ class PagedPlan:
             raise ValueError("Plan tensors must be contiguous int32 tensors on one device")
         if t.ndim != 2 or 0 in t.shape or n.shape != t.shape[:1] or s.shape != (t.shape[0] + 1,):
             raise ValueError("A plan holds page_table [B, width], key_lengths [B] and query_starts [B + 1]")
+        _nonnegative_integer("most_new", self.most_new)
 
     @classmethod
     def create(cls, page_table, key_lengths, query_starts, *, page_size=64, pages=None):
@@ -136,10 +140,12 @@ class PagedPlan:
             raise ValueError("A sequence has more new tokens than keys")
         if pages is not None and bool((page_table >= pages).any()):
             raise ValueError("page_table names a page outside the cache")
-        return plan
+        return cls(plan.page_table, plan.key_lengths, plan.query_starts,
+                   int((query_starts[1:] - query_starts[:-1]).max()))
 
     def to(self, device):
-        return PagedPlan(*(x.to(device) for x in (self.page_table, self.key_lengths, self.query_starts)))
+        return PagedPlan(*(x.to(device) for x in (self.page_table, self.key_lengths, self.query_starts)),
+                         self.most_new)
 
 
 def _check(cache, plan, *xs):
@@ -246,13 +252,13 @@ def _attend(q, cache, plan, rule, scale, out):
     fresh = out is None
     word = monitor(q.device).word()
     keep, ws, size = workspace("solattn_paged_workspace_bytes",
-                               (N, B, Hq, cache.heads, D, cache.page_size, width, *rule), q.device)
+                               (N, B, Hq, cache.heads, D, cache.page_size, width, plan.most_new, *rule), q.device)
     if fresh:
         out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
     rc = _lib.load().solattn_paged_attention(
         q.data_ptr(), N, Hq, cache.heads, D, q.stride(0), q.stride(1), *cache._args,
         plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(), plan.query_starts.data_ptr(), B,
-        *rule, scale, int(fresh), ws, size, out.data_ptr(), word,
+        plan.most_new, *rule, scale, int(fresh), ws, size, out.data_ptr(), word,
         torch.cuda.current_stream(q.device).cuda_stream)
     _lib.check(rc, "solattn_paged_attention")
     return out

@@ -129,12 +129,12 @@ def test_window_entry_point_rejects(bad, code):
 
 def _paged(**over):
     a = dict(q=16, N=2, Hq=4, Hkv=2, D=64, qs=(256, 64), k=16, v=16, ks=None, vs=None, pages=4, page_size=16,
-             table=16, width=3, lengths=16, starts=16, B=2, window=0, ahead=-1, sinks=0, scale=0.125, ws=None,
-             size=0, out=16)
+             table=16, width=3, lengths=16, starts=16, B=2, most=0, window=0, ahead=-1, sinks=0, scale=0.125,
+             ws=None, size=0, out=16)
     a.update(over)
     return _lib.load().solattn_paged_attention(
         a["q"], a["N"], a["Hq"], a["Hkv"], a["D"], *a["qs"], a["k"], a["v"], a["ks"], a["vs"], a["pages"],
-        a["page_size"], a["table"], a["width"], a["lengths"], a["starts"], a["B"], a["window"], a["ahead"],
+        a["page_size"], a["table"], a["width"], a["lengths"], a["starts"], a["B"], a["most"], a["window"], a["ahead"],
         a["sinks"], a["scale"], 0, a["ws"], a["size"], a["out"], None, None)
 
 
@@ -143,6 +143,7 @@ def _paged(**over):
     (dict(ks=16), -1), (dict(table=None), -1), (dict(starts=None), -1), (dict(pages=0), -1), (dict(width=0), -1),
     (dict(width=1 << 21), -1), (dict(qs=(255, 64)), -1), (dict(Hq=3), -1), (dict(scale=-1.0), -1),
     (dict(width=60000), -1),  # (needs a workspace)
+    (dict(most=-1), -1), (dict(pages=(1 << 30) + 1), -1),
 ])
 def test_paged_entry_point_rejects(bad, code):
     assert _paged(**bad) == code
@@ -168,7 +169,7 @@ def test_workspace_sizes():
     L = _lib.load()
     assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 2, 64, 0, 0, 0) == 0
     assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 3, 64, 0, 0, 0) == -1
-    size = L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 16, 0, 0, 0)
+    size = L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 16, 1, 0, 0, 0)
     assert size > 0 and size % (16 * 130 * 4) == 0
     # A window bounds what is split, however wide the table is.
-    assert L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 1 << 18, 64, 0, 4) == 0
+    assert L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 1 << 18, 1, 64, 0, 4) == 0
