@@ -110,13 +110,25 @@ struct Ctl {
   volatile int* abort;
   int32_t* status;
 };
-__device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, const Ctl& c) {
-  if (mbar_try_wait(bar, parity)) return true;
+// One poll, without a suspend hint (a wait that is over already costs a third of one with it).
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The whole warp waits; the vote keeps it together whatever the lanes saw.
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, const Ctl& c) {
   const long long t0 = clock64();
   while (true) {
-    if (*c.abort) return false;
-    if (mbar_try_wait(bar, parity)) return true;
-    if (clock64() - t0 > kWaitLimitCycles) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *c.abort != 0)) return false;
+    if (__any_sync(0xffffffffu, clock64() - t0 > kWaitLimitCycles)) {
       *c.abort = 1;
       note(c.status, kStatusWaitTimeout);
       return false;
@@ -124,8 +136,8 @@ __device__ __forceinline__ bool wait1(uint32_t bar, uint32_t parity, const Ctl& 
   }
 }
 __device__ __forceinline__ bool waitw(uint32_t bar, uint32_t parity, const Ctl& c) {
-  const bool ok = wait1(bar, parity, c);
-  return __all_sync(0xffffffffu, ok);
+  if (__all_sync(0xffffffffu, poll(bar, parity))) return true;
+  return wait_long(bar, parity, c);
 }
 __device__ __forceinline__ void wait_quiet(uint32_t bar, uint32_t parity) {
   const long long t0 = clock64();
@@ -172,14 +184,13 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
 // Columns [0, n) of a 32-column word of a tile, n clamped.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
-// Finds item `i` of the launch.  Items run head by head (those in flight share K/V in the L2), within
-// a head from the last row tile to the first (under a causal rule the longest first).
+// Finds unit `i` of the launch: an item, or one of the splits of an item from number `first` on.
 template <int D>
 __device__ __forceinline__ bool find_item(const SeqParams& p, int64_t i, int lane, Item& it) {
-  const int64_t per_head = (int64_t)p.slots * p.splits;
-  it.h = (int)(i / per_head);
-  const int r = (int)(i % per_head);
-  const int slot = p.slots - 1 - r / p.splits, split = r % p.splits;
+  const int64_t r = i - p.first;
+  const int id = r < 0 ? (int)i : p.first + (int)(r / p.splits), split = r < 0 ? 0 : (int)(r % p.splits);
+  int slot;
+  chunk_item(p, id, it.h, slot);
   const Seq sq = find_seq<kItemRows>(p, slot, lane);
   it.b = sq.b;
   if (sq.b < 0 || !p.takes(sq.n)) return false;
@@ -201,11 +212,11 @@ __device__ __forceinline__ bool find_item(const SeqParams& p, int64_t i, int lan
     it.stage[1].sink = it.stage[1].from = it.stage[1].to = 0;
   }
   const int total = it.all.count();
-  it.splits = max(1, min(p.splits, (total + p.unit - 1) / p.unit));
+  it.splits = r < 0 ? 1 : max(1, min(p.splits, (total + p.unit - 1) / p.unit));
   if (split >= it.splits) return false;
   it.c0 = (int)((int64_t)total * split / it.splits);
   it.c1 = (int)((int64_t)total * (split + 1) / it.splits);
-  it.part = (slot * p.Hkv + it.h) * p.splits + split;
+  it.part = (id - p.first) * p.splits + split;
   return true;
 }
 
@@ -512,7 +523,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         if (lane == 0) mbar_arrive(bar(C::O_FREE + st));
       }
       if (partial && mine_row) {
-        float2* ml = reinterpret_cast<float2*>(p.part + (int64_t)p.slots * p.Hkv * p.splits * kItemRows * D) + prow;
+        float2* ml = reinterpret_cast<float2*>(p.part + (int64_t)(p.slots * p.Hkv - p.first) * p.splits * kItemRows * D) + prow;
         *ml = make_float2(m_run, l_run);
       }
       if (!it.careful && __any_sync(0xffffffffu, mine_row && check != 0.f) && lane == 0)
@@ -771,7 +782,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
       }
     } else if (warp == kItemWarp) {
       // ---------------------------------------------------------------- items and Q
-      const int64_t total = (int64_t)p.slots * p.splits * p.Hkv;
+      const int64_t total = p.first + (int64_t)(p.slots * p.Hkv - p.first) * p.splits;
       const int64_t per_cta = (total + gridDim.x - 1) / gridDim.x;
       int shift = 0;  // redo bits cover 2^shift items when a CTA has more than kRedoBits
       while ((per_cta >> shift) > kRedoBits - 1) ++shift;
@@ -984,11 +995,12 @@ cudaError_t launch_chunk_kv(const SeqParams& p, cudaStream_t stream) {
   err = cudaGetDevice(&dev);
   if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (err != cudaSuccess) return err;
-  const int64_t items = (int64_t)p.slots * p.Hkv * p.splits;
-  kernel<<<(unsigned)(items < sms ? items : sms), C::kThreads, C::kBytes, stream>>>(p, tmK, tmV);
+  const int64_t split_items = (int64_t)p.slots * p.Hkv - p.first;
+  const int64_t units = p.first + split_items * p.splits;
+  kernel<<<(unsigned)(units < sms ? units : sms), C::kThreads, C::kBytes, stream>>>(p, tmK, tmV);
   err = cudaGetLastError();
-  if (err != cudaSuccess || p.splits == 1) return err;
-  join_kernel<D, kItemRows, kKeys><<<dim3((unsigned)((int64_t)p.slots * p.Hkv), kItemRows / 16), kJoinThreads, 0, stream>>>(p);
+  if (err != cudaSuccess || p.splits == 1 || split_items == 0) return err;
+  join_kernel<D, kItemRows, kKeys><<<dim3((unsigned)split_items, kItemRows / 16), kJoinThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 

@@ -14,7 +14,13 @@ constexpr int kJoinThreads = 128;
 template <int D, int R, int T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = (int)(blockIdx.x % p.Hkv), slot = (int)(blockIdx.x / p.Hkv);
+  int h, slot;
+  if (R == 16) {  // rows.cu
+    h = (int)(blockIdx.x % p.Hkv);
+    slot = (int)(blockIdx.x / p.Hkv);
+  } else {
+    chunk_item(p, p.first + (int)blockIdx.x, h, slot);
+  }
   const Seq sq = find_seq<R>(p, slot, lane);
   if (sq.b < 0 || !p.takes(sq.n)) return;
   const int r_base = sq.tile * R, off = sq.L - sq.n;
@@ -22,8 +28,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const KeyTiles kt = key_tiles<T>(p, sq.L, off + r_base / p.G, off + (r_base + rows - 1) / p.G);
   const int ns = max(1, min(p.splits, (kt.count() + p.unit - 1) / p.unit));
   if (ns == 1) return;
-  const int64_t unit0 = ((int64_t)slot * p.Hkv + h) * p.splits;
-  const float2* ml0 = reinterpret_cast<const float2*>(p.part + (int64_t)p.slots * p.Hkv * p.splits * R * D);
+  const int64_t unit0 = (int64_t)blockIdx.x * p.splits;
+  const float2* ml0 = reinterpret_cast<const float2*>(p.part + (int64_t)gridDim.x * p.splits * R * D);
   constexpr int kPer = D / 32;  // dims of a lane
   const int r0 = 16 * blockIdx.y, r1 = min(rows, r0 + 16);
   for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {

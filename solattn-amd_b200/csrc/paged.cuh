@@ -40,7 +40,8 @@ struct SeqParams {
   int32_t* status;     // device-accessible word (pinned host memory) or nullptr
   int B, N, Hq, Hkv, G, Tq, Tk;  // N: rows of q over all sequences (B * Tq when contiguous)
   int window, ahead, sinks;
-  int slots, splits, unit;  // row tiles over all sequences; splits of a tile; keys tiles per split
+  int slots, splits, unit;  // row tiles over all sequences; splits of a tile; key tiles per split
+  int first;                // items (a slot and a K/V head) from this number on are split
   int zero_tail;            // write zeros to the rows behind the last sequence
   int min_new, max_new;     // new tokens of the sequences that this launch takes
   float scale_log2;         // softmax scale * log2(e)
@@ -133,6 +134,13 @@ __device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) 
   }
   s.L = L;
   return s;
+}
+
+// Item number `id` of the chunk kernel: head by head (the items in flight share K and V in the L2),
+// within a head from the last row tile to the first (under a causal rule the longest first).
+__device__ __forceinline__ void chunk_item(const SeqParams& p, int id, int& h, int& slot) {
+  h = id / p.slots;
+  slot = p.slots - 1 - id % p.slots;
 }
 
 // The keys that a query at position pos sees: [lo, hi] and [0, min(sinks - 1, hi)].

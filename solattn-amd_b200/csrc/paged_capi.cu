@@ -44,12 +44,13 @@ bool rule_ok(const Rule& r) {
 // keys over `splits` CTAs of at least `unit` 16-key chunks.
 struct Split {
   int64_t slots, splits, unit;
+  int64_t first = 0;  // items before this one are not split
 };
 Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t cap, bool paged,
                  const Rule& r) {
   Split s;
   const int64_t G = Hq / Hkv;
-  s.slots = paged ? N * G / 16 + B : B * cdiv(Tq * G, 16);
+  s.slots = paged && B > 1 ? N * G / 16 + B : B * cdiv((paged ? N : Tq) * G, 16);
   int64_t keys = cap;
   if (r.window > 0 && r.lookahead >= 0) {
     const int64_t span = r.window + r.lookahead + r.sinks + 16 + 48;
@@ -65,29 +66,38 @@ Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int6
   return s;
 }
 
-// How the chunk kernel divides a call: tiles of 256 rows and key splits of at least `unit` 128-key
-// tiles.  Its CTAs work through equal shares of the items, so the time is about (items per SM, rounded
-// up) * (tiles per item + 3), in key tiles; 3 is what starting and ending an item costs, and a join
-// about 4.  The split with the least such time is taken (the lengths being known only as bounds).
+// How the chunk kernel divides a call: items (tiles of 256 rows of a K/V head), the last of them split
+// over the keys.  Its CTAs take the items in turn, so the time is about (items per SM, rounded up) *
+// (tiles of an item + 3), in key tiles; 3 is what starting and ending an item costs, and a join about
+// 4.  Either every item is split, or those that do not fill a round of the SMs; what takes the least
+// such time is done (the lengths being known only as bounds).
 Split chunk_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t cap, bool paged,
                   const Rule& r) {
   Split s;
   const int64_t G = Hq / Hkv;
-  s.slots = paged ? N * G / 256 + B : B * cdiv(Tq * G, 256);
+  const bool known = !paged || B == 1;  // which slots hold rows
+  s.slots = known ? B * cdiv((paged ? N : Tq) * G, 256) : N * G / 256 + B;
   int64_t keys = cap;
   if (r.window > 0 && r.lookahead >= 0) {
     const int64_t span = r.window + r.lookahead + r.sinks + 256 / G + 1;
     if (span < keys) keys = span;
   }
   const int64_t tiles = cdiv(keys, 128) + 1;
-  const int64_t items = Hkv * (paged ? cdiv(N * G, 256) + B / 2 : s.slots);
-  int64_t best = 0;
+  // Of a packed call's slots, which have room for every way to cut N rows into B sequences, about so
+  // many hold rows.
+  const int64_t all = s.slots * Hkv, items = known ? all : Hkv * (cdiv(N * G, 256) + B / 2);
+  int64_t best = cdiv(items, kSms) * (tiles + 3);
+  s.first = all;
   s.splits = 1;
-  for (int64_t n = 1; n <= 64 && n <= tiles; ++n) {
-    const int64_t time = cdiv(items * n, kSms) * (cdiv(tiles, n) + 3) + (n > 1 ? 4 : 0);
-    if (n == 1 || time < best) {
-      best = time;
-      s.splits = n;
+  for (int whole = 0; whole < (known ? 2 : 1); ++whole) {
+    const int64_t rounds = whole ? items / kSms : 0, rest = items - rounds * kSms;
+    for (int64_t n = 2; n <= 64 && n <= tiles && rest > 0; ++n) {
+      const int64_t time = rounds * (tiles + 3) + cdiv(rest * n, kSms) * (cdiv(tiles, n) + 3) + 4;
+      if (time < best) {
+        best = time;
+        s.splits = n;
+        s.first = whole ? all - rest : 0;
+      }
     }
   }
   s.unit = cdiv(tiles, s.splits);
@@ -95,7 +105,7 @@ Split chunk_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int
 }
 
 int64_t split_bytes(const Split& s, int64_t tile_rows, int64_t Hkv, int64_t D) {
-  return s.splits > 1 ? s.slots * Hkv * s.splits * tile_rows * (D + 2) * 4 : 0;
+  return s.splits > 1 ? (s.slots * Hkv - s.first) * s.splits * tile_rows * (D + 2) * 4 : 0;
 }
 
 // Which kernels a call takes.  The few-rows kernel reads its keys once per 16 rows, the chunk kernel
@@ -168,6 +178,7 @@ int run(SeqParams& p, int64_t D, int kv, const Choice& c, void* workspace, int64
     x.slots = (int)s.slots;
     x.splits = (int)s.splits;
     x.unit = (int)s.unit;
+    x.first = (int)s.first;
     x.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (many ? c.rows_bytes : 0));
     x.min_new = many && c.few ? (int)least : 0;
     x.max_new = !many && c.many ? (int)least - 1 : 0x7fffffff;
