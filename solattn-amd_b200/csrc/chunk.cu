@@ -19,6 +19,7 @@
 // again at the end, carefully: warp 10 (or the converters) zeroes every V row that is not finite and
 // the softmax warps add what each row sees of it.
 #include <cstring>
+#include <type_traits>
 
 #include "join.cuh"
 #include "sm100.cuh"
@@ -36,6 +37,7 @@ constexpr int kKeys = 128;      // keys of a tile
 constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kCheckWarp = 10, kItemWarp = 11, kConvWarp0 = 12;
 constexpr int kConvWarps = 4;
+constexpr int kConvBatch = 2;  // pieces that a converter thread reads before it writes (1, 2, 4: 257, 241, 247 us)
 constexpr int kBox = kKeys * 128;  // 128 rows x 64 BF16 columns, 128-byte swizzled
 constexpr uint32_t kTmemCols = 512, kTmemS = 0, kTmemO = 256;  // stage s at + 128 s
 constexpr int kRedoBits = 1024;
@@ -181,6 +183,14 @@ __device__ __forceinline__ uint32_t tile_off(int r, int c) {
   return (uint32_t)((c >> 3) * kBox + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// E4M3 tiles hold the dims of a group of four in the order 0, 2, 1, 3, which is how a word of codes
+// falls apart without byte moves: K, and Q to match, along the contraction; V, and so O's columns.  The
+// order is its own inverse.
+template <int KV>
+__host__ __device__ constexpr int col_of(int d) {
+  return KV == kPagedE4m3 ? (d & ~3) | ((d & 1) << 1) | ((d >> 1) & 1) : d;
+}
+
 // Columns [0, n) of a 32-column word of a tile, n clamped.
 __device__ __forceinline__ uint32_t below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
@@ -299,22 +309,25 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
     }
     bool ok = true;
     for (int k = 0; ok; ++k) {
-      Item it;
-      if (!next_item(k, it)) break;
+      // (The description stays in shared memory until the item is released: registers are short here.)
+      if (!waitw(bar(C::ITEM_FULL + (k & 1)), (uint32_t)(k >> 1) & 1u, ctl)) break;
+      const Item& it = *item_slot(k & 1);
+      if (it.b < 0) break;
       const int off = it.L - it.n;
       const int wrow = st * kStageRows + quarter * 32;  // first row of the warp within the item
       const bool warp_rows = wrow < it.rows;
-      const int row = min(wrow + lane, it.rows - 1);
-      const int tok = (it.row0 + row) / p.G;
-      const int hi = key_high(p, it.L, off + tok), lo = key_low(p, off + tok);
+      const int pos = off + (it.row0 + min(wrow + lane, it.rows - 1)) / p.G;
+      const int hi = key_high(p, it.L, pos), lo = key_low(p, pos);
       // What all rows of the warp see, and what any of them does.
       const int all_hi = __shfl_sync(0xffffffffu, hi, 0), all_lo = __shfl_sync(0xffffffffu, lo, 31);
       const int any_hi = __shfl_sync(0xffffffffu, hi, 31), any_lo = __shfl_sync(0xffffffffu, lo, 0);
-      const KeyTiles mine = it.stage[st];
+      const KeyTiles mine = it.stage[st], list = it.all;
+      const int c0 = it.c0, c1 = it.c1;
+      const bool careful = it.careful != 0;
       float m_run = -INFINITY, l_run = 0.f;
       bool has = false;
-      for (int i = it.c0; i < it.c1; ++i) {
-        const int t = it.all.at(i);
+      for (int i = c0; i < c1; ++i) {
+        const int t = list.at(i);
         if (!needs(mine, t)) continue;
         const int kb = t * kKeys;
         const bool first = !has;
@@ -420,9 +433,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           }
         }
         tmem_wait_st();
-        if (it.careful) {
+        if (careful) {
           // V rows that were zeroed for not being finite: add what this row sees of them.
-          const int gi = g + i - it.c0, slot = gi % C::kSlots;
+          const int gi = g + i - c0, slot = gi % C::kSlots;
           if (!waitw(bar(C::V_OK + slot), (uint32_t)(gi / C::kSlots) & 1u, ctl) ||
               (!first && !waitw(bar(C::PV_DONE + st), (uint32_t)ns & 1u, ctl))) {
             ok = false;
@@ -432,18 +445,18 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
 #pragma unroll 1
           for (int key = 0; key < kKeys; ++key) {
             if (!((bad[4 * slot + (key >> 5)] >> (key & 31)) & 1u)) continue;
-            const int pos = kb + key;
+            const int at = kb + key;
             const uint32_t pair = tmem_ld1(tS + (uint32_t)(key >> 1));
             tmem_wait_ld();
             const float pv = __uint_as_float((key & 1) ? (pair & 0xffff0000u) : (pair << 16));
-            const bool see = pos <= hi && (pos >= lo || pos < p.sinks);
+            const bool see = at <= hi && (at >= lo || at < p.sinks);
             const uint8_t* src;
             float f = 1.f;
             if (KV == kStrided) {
-              src = p.v + ((int64_t)it.b * p.v_sB + (int64_t)pos * p.v_sT + (int64_t)it.h * p.v_sH) * 2;
+              src = p.v + ((int64_t)it.b * p.v_sB + (int64_t)at * p.v_sT + (int64_t)it.h * p.v_sH) * 2;
             } else {
-              const int page = page_of(p, it.b, pos);
-              const int64_t r = (((int64_t)page * p.Hkv + it.h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+              const int page = page_of(p, it.b, at);
+              const int64_t r = (((int64_t)page * p.Hkv + it.h) << p.page_shift) + (at & ((1 << p.page_shift) - 1));
               src = p.v + r * (KV == kPagedE4m3 ? D : 2 * D);
               if (KV == kPagedE4m3) f = e8m0_value(p.v_scale[r]);
             }
@@ -454,7 +467,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
               tmem_wait_ld();
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const int d = 16 * c + j;
+                const int d = 16 * c + col_of<KV>(j);
                 const float x = KV == kPagedE4m3
                                     ? e4m3_value(src[d]) * f
                                     : __uint_as_float((uint32_t) reinterpret_cast<const uint16_t*>(src)[d] << 16);
@@ -470,7 +483,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         if (lane == 0) mbar_arrive(bar(C::P_FULL + st));
       }
       if (!ok) break;
-      g += it.c1 - it.c0;
+      g += c1 - c0;
       // ---- the item's rows: O / l (or the partial O, m, l), then O = 0 for the next item
       if (has && !waitw(bar(C::PV_DONE + st), (uint32_t)(ns - 1) & 1u, ctl)) break;
       tc_fence_after();
@@ -478,8 +491,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
       const bool any = hi >= 0 && (hi >= lo || p.sinks > 0);
       const float inv = any ? 1.f / l_run : 0.f;
       const bool partial = it.splits > 1;
+      const int row = it.row0 + min(wrow + lane, it.rows - 1), tok = row / p.G;
       const int64_t prow = (int64_t)it.part * kItemRows + wrow + lane;
-      __nv_bfloat16* dst = p.out + ((int64_t)(it.start + tok) * p.Hq + it.h * p.G + (it.row0 + row) % p.G) * D;
+      __nv_bfloat16* dst = p.out + ((int64_t)(it.start + tok) * p.Hq + it.h * p.G + row % p.G) * D;
       float check = l_run * 0.f;  // not zero where a value is not finite
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -498,13 +512,15 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
             float4* d4 = reinterpret_cast<float4*>(p.part + prow * D + 32 * c);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              d4[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]),
-                                  __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+              d4[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[col_of<KV>(4 * j + 1)]),
+                                  __uint_as_float(o[col_of<KV>(4 * j + 2)]), __uint_as_float(o[4 * j + 3]));
           } else {
             uint32_t w[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              w[j] = any ? pack_bf16(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv) : 0u;
+              w[j] = any ? pack_bf16(__uint_as_float(o[col_of<KV>(2 * j)]) * inv,
+                                   __uint_as_float(o[col_of<KV>(2 * j + 1)]) * inv)
+                       : 0u;
             uint4* d4 = reinterpret_cast<uint4*>(dst + 32 * c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) d4[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
@@ -526,7 +542,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         float2* ml = reinterpret_cast<float2*>(p.part + (int64_t)(p.slots * p.Hkv - p.first) * p.splits * kItemRows * D) + prow;
         *ml = make_float2(m_run, l_run);
       }
-      if (!it.careful && __any_sync(0xffffffffu, mine_row && check != 0.f) && lane == 0)
+      if (!careful && __any_sync(0xffffffffu, mine_row && check != 0.f) && lane == 0)
         atomicOr(&redo[it.redo >> 5], 1u << (it.redo & 31));
       release_item(k);
     }
@@ -833,16 +849,42 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           for (int j = 0; j < kItemRows / 32; ++j) {
             const int r = it.row0 + min(32 * j + lane, it.rows - 1);
             const int64_t mo = (int64_t)(r / p.G) * p.q_sT + (int64_t)(r % p.G) * p.q_sH;
+            if constexpr (!C::kCodes) {
 #pragma unroll
-            for (int x = 0; x < 32 / kPer; ++x) {
-              const int rr = x * kPer + lane / (D / 8);
-              const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
-              const int row = 32 * j + rr;
-              cp_async16(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
-                         base + o + 8 * c, row < it.rows ? 16 : 0);
+              for (int x = 0; x < 32 / kPer; ++x) {
+                const int rr = x * kPer + lane / (D / 8);
+                const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
+                const int row = 32 * j + rr;
+                cp_async16(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
+                           base + o + 8 * c, row < it.rows ? 16 : 0);
+              }
+            } else {  // through registers, into the order of the converted K tiles
+#pragma unroll
+              for (int x0 = 0; x0 < 32 / kPer; x0 += 4) {
+                uint4 v[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const int rr = (x0 + x) * kPer + lane / (D / 8);
+                  const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
+                  v[x] = 32 * j + rr < it.rows ? __ldg(reinterpret_cast<const uint4*>(base + o + 8 * c))
+                                               : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const int row = 32 * j + (x0 + x) * kPer + lane / (D / 8);
+                  sts128(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
+                         make_uint4(__byte_perm(v[x].x, v[x].y, 0x5410), __byte_perm(v[x].x, v[x].y, 0x7632),
+                                    __byte_perm(v[x].z, v[x].w, 0x5410), __byte_perm(v[x].z, v[x].w, 0x7632)));
+                }
+              }
             }
           }
-          cp_async_mbar_arrive_noinc(bar(C::Q_FULL + qb));
+          if constexpr (C::kCodes) {
+            fence_proxy_async_smem();
+            mbar_arrive(bar(C::Q_FULL + qb));
+          } else {
+            cp_async_mbar_arrive_noinc(bar(C::Q_FULL + qb));
+          }
           ++k;
         }
       }
@@ -856,7 +898,10 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
     } else if constexpr (C::kCodes) {
       // ---------------------------------------------------------------- E4M3 codes to BF16 tiles
       const int ct = tid - kConvWarp0 * 32;
-      constexpr int kPieces = D / 16;  // 16-code pieces of a row
+      constexpr int kPieces = D / 16;           // 16-code pieces of a row
+      constexpr int kRowStep = 128 / kPieces;   // rows that the converters take at a time
+      const int r0 = ct / kPieces, piece = ct % kPieces;
+      const uint32_t to0 = tile_off(r0, 2 * piece), to1 = tile_off(r0, 2 * piece + 1);
       int g = 0;
       bool ok = true;
       for (int k = 0; ok; ++k) {
@@ -877,61 +922,77 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
             const uint32_t src = sbase + (uint32_t)(C::kCode + cs * C::kCodeTile);
             const uint8_t* sc = smem + C::kScale + cs * kKeys;
             const uint32_t dst = sbase + (uint32_t)((z ? C::kV : C::kK) + sl * C::kTile);
-#pragma unroll 2
-            for (int x = 0; x < kKeys * kPieces / 128; ++x) {
-              const int q = x * 128 + ct, r = q / kPieces, c = q % kPieces;
-              const bool behind = unseen(it, p.sinks, kb + r);
-              const uint4 w4 = lds128v(src + (uint32_t)(r * D + 16 * c));
-              const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-              const uint32_t e = behind ? 0u : sc[r];
-              uint32_t y[8];
-              // value = code fields * 2^120 * 2^(e - 127): one factor where it is a BF16.
-              uint32_t f = e == 255u ? 0x7fc0u : e <= 134u ? (e + 120u) << 7 : 0x7f00u;
-              f |= f << 16;
-              uint32_t nan = 0u;
+            // Most tiles are plain: every row is seen by somebody, and the item is not a careful one.
+            auto convert = [&](auto plain) {
+#pragma unroll 1
+              for (int x0 = 0; x0 < kKeys / kRowStep; x0 += kConvBatch) {
+                uint4 wb[kConvBatch];  // a batch's codes and scales, before any of its stores
+                uint32_t eb[kConvBatch];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                nan |= e4m3_nan_bytes(w[j]);
-                y[2 * j] = bf16x2_mul(e4m3_fields(__byte_perm(w[j], 0u, 0x1404)), f);
-                y[2 * j + 1] = bf16x2_mul(e4m3_fields(__byte_perm(w[j], 0u, 0x3424)), f);
-              }
-              if (e > 134u && e < 255u) {
-                uint32_t f2 = (e - 7u) << 7;
-                f2 |= f2 << 16;
+                for (int x = 0; x < kConvBatch; ++x) {
+                  wb[x] = lds128v(src + (uint32_t)((r0 + kRowStep * (x0 + x)) * D + 16 * piece));
+                  eb[x] = sc[r0 + kRowStep * (x0 + x)];
+                }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = bf16x2_mul(y[j], f2);
-              }
-              if (nan) {  // (rare) NaN codes: element by element
+                for (int xb = 0; xb < kConvBatch; ++xb) {
+                  const int x = x0 + xb, r = r0 + kRowStep * x;
+                  const uint32_t w[4] = {wb[xb].x, wb[xb].y, wb[xb].z, wb[xb].w};
+                  const uint32_t e = eb[xb];
+                  uint32_t y[8];
+                  // value = code fields * 2^120 * 2^(e - 127): one factor where it is a BF16.
+                  uint32_t f = e <= 134u ? (e + 120u) << 7 : 0x7f00u;
+                  f |= f << 16;
+                  uint32_t top = 0u;  // the largest fields: 0x7f0 where a code is NaN
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const uint32_t two = w[j >> 1] >> (16 * (j & 1));
-                  if ((two & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
-                  if ((two & 0x7f00u) == 0x7f00u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
+                  for (int j = 0; j < 4; ++j) {
+                    const uint32_t odd = (w[j] >> 4) & 0x07f007f0u, even = (w[j] << 4) & 0x07f007f0u;
+                    top = __vimax3_u16x2(top, odd, even);
+                    y[2 * j] = bf16x2_mul(even | ((w[j] << 8) & 0x80008000u), f);
+                    y[2 * j + 1] = bf16x2_mul(odd | (w[j] & 0x80008000u), f);
+                  }
+                  if (e > 134u || (top >> 16) == 0x7f0u || (top & 0xffffu) == 0x7f0u) {
+                    // (Rare) scales above 2^7, and NaN codes or scale.
+                    uint32_t f2 = e > 134u && e < 255u ? (e - 7u) << 7 : e == 255u ? 0x7fc0u : 0x3f80u;
+                    f2 |= f2 << 16;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                      y[j] = bf16x2_mul(y[j], f2);
+                      const uint32_t two = (j & 1) ? w[j >> 1] >> 8 : w[j >> 1];  // codes in bytes 0 and 2
+                      if ((two & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
+                      if ((two & 0x7f0000u) == 0x7f0000u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
+                    }
+                  }
+                  if constexpr (!decltype(plain)::value) {
+                    if (unseen(it, p.sinks, kb + r)) {
+#pragma unroll
+                      for (int j = 0; j < 8; ++j) y[j] = 0u;
+                    }
+                    if (z && it.careful) {  // a row's pieces lie in one warp: all of it becomes zero
+                      uint32_t acc = 0u;
+#pragma unroll
+                      for (int j = 0; j < 8; ++j) acc = bf16x2_fma(y[j], 0u, acc);
+                      const uint32_t wrong = __ballot_sync(0xffffffffu, (acc & 0x7fff7fffu) != 0u);
+                      const bool row_wrong = ((wrong >> (lane & ~(kPieces - 1))) & ((1u << kPieces) - 1u)) != 0u;
+                      uint32_t* word = const_cast<uint32_t*>(&bad[4 * sl + (r >> 5)]);
+                      if (piece == 0) {
+                        if (row_wrong) atomicOr(word, 1u << (r & 31));
+                        else atomicAnd(word, ~(1u << (r & 31)));
+                      }
+                      if (row_wrong) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) y[j] = 0u;
+                      }
+                    }
+                  }
+                  // (Rows of one lane differ by multiples of 8: the swizzle stays.)
+                  sts128(dst + to0 + (uint32_t)(kRowStep * 128 * x), make_uint4(y[0], y[1], y[2], y[3]));
+                  sts128(dst + to1 + (uint32_t)(kRowStep * 128 * x), make_uint4(y[4], y[5], y[6], y[7]));
                 }
               }
-              if (behind) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = 0u;
-              }
-              if (z && it.careful) {  // a row's pieces lie in one warp: all of it becomes zero
-                uint32_t acc = 0u;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) acc = bf16x2_fma(y[j], 0u, acc);
-                const uint32_t wrong = __ballot_sync(0xffffffffu, (acc & 0x7fff7fffu) != 0u);
-                const bool row_wrong = ((wrong >> (lane & ~(kPieces - 1))) & ((1u << kPieces) - 1u)) != 0u;
-                uint32_t* word = const_cast<uint32_t*>(&bad[4 * sl + (r >> 5)]);
-                if (c == 0) {
-                  if (row_wrong) atomicOr(word, 1u << (r & 31));
-                  else atomicAnd(word, ~(1u << (r & 31)));
-                }
-                if (row_wrong) {
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) y[j] = 0u;
-                }
-              }
-              sts128(dst + tile_off(r, 2 * c), make_uint4(y[0], y[1], y[2], y[3]));
-              sts128(dst + tile_off(r, 2 * c + 1), make_uint4(y[4], y[5], y[6], y[7]));
-            }
+            };
+            const bool edge = kb + kKeys - 1 > it.high || (kb < it.low && kb + kKeys > p.sinks);
+            if (edge || it.careful) convert(std::false_type{});
+            else convert(std::true_type{});
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
