@@ -66,7 +66,7 @@ struct ChunkCfg {
   static constexpr int kBars = kScale + kCodeSlots * kKeys;
   // Barriers.
   static constexpr int ITEM_FULL = 0, ITEM_EMPTY = 2, Q_FULL = 4, Q_EMPTY = 6, S_FULL = 8, P_FULL = 10,
-                       PV_DONE = 12, O_FREE = 14, DRAIN = 16, K_FULL = 17, K_EMPTY = K_FULL + kSlots,
+                       PV_DONE = 12, O_FREE = 14, DRAIN = 16, Q_RAW = 17 /* E4M3 */, K_FULL = 19, K_EMPTY = K_FULL + kSlots,
                        V_FULL = K_EMPTY + kSlots, V_OK = V_FULL + kSlots, V_EMPTY = V_OK + kSlots,
                        CODE_FULL = V_EMPTY + kSlots, CODE_EMPTY = CODE_FULL + kCodeSlots,
                        NBARS = CODE_EMPTY + kCodeSlots;
@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
     for (int i = 0; i < C::NBARS; ++i) {
       uint32_t count = 1;
       if (i >= C::ITEM_EMPTY && i < C::ITEM_EMPTY + 2) count = 3 + kSoftmaxWarps + (C::kCodes ? kConvWarps - 1 : 0);
-      if (i >= C::Q_FULL && i < C::Q_FULL + 2) count = 32;
+      if (i >= C::Q_FULL && i < C::Q_FULL + 2) count = C::kCodes ? kConvWarps : 32;
+      if (i >= C::Q_RAW && i < C::Q_RAW + 2) count = 32;
       if ((i >= C::P_FULL && i < C::P_FULL + 2) || (i >= C::O_FREE && i < C::O_FREE + 2)) count = 4;
       if (C::kCodes && ((i >= C::K_FULL && i < C::K_FULL + C::kSlots) || (i >= C::V_OK && i < C::V_OK + C::kSlots)))
         count = kConvWarps;
@@ -849,42 +850,16 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           for (int j = 0; j < kItemRows / 32; ++j) {
             const int r = it.row0 + min(32 * j + lane, it.rows - 1);
             const int64_t mo = (int64_t)(r / p.G) * p.q_sT + (int64_t)(r % p.G) * p.q_sH;
-            if constexpr (!C::kCodes) {
 #pragma unroll
-              for (int x = 0; x < 32 / kPer; ++x) {
-                const int rr = x * kPer + lane / (D / 8);
-                const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
-                const int row = 32 * j + rr;
-                cp_async16(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
-                           base + o + 8 * c, row < it.rows ? 16 : 0);
-              }
-            } else {  // through registers, into the order of the converted K tiles
-#pragma unroll
-              for (int x0 = 0; x0 < 32 / kPer; x0 += 4) {
-                uint4 v[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const int rr = (x0 + x) * kPer + lane / (D / 8);
-                  const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
-                  v[x] = 32 * j + rr < it.rows ? __ldg(reinterpret_cast<const uint4*>(base + o + 8 * c))
-                                               : make_uint4(0, 0, 0, 0);
-                }
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const int row = 32 * j + (x0 + x) * kPer + lane / (D / 8);
-                  sts128(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
-                         make_uint4(__byte_perm(v[x].x, v[x].y, 0x5410), __byte_perm(v[x].x, v[x].y, 0x7632),
-                                    __byte_perm(v[x].z, v[x].w, 0x5410), __byte_perm(v[x].z, v[x].w, 0x7632)));
-                }
-              }
+            for (int x = 0; x < 32 / kPer; ++x) {
+              const int rr = x * kPer + lane / (D / 8);
+              const int64_t o = __shfl_sync(0xffffffffu, mo, rr);
+              const int row = 32 * j + rr;
+              cp_async16(sq + (uint32_t)((row / kStageRows) * C::kTile) + tile_off(row % kStageRows, c),
+                         base + o + 8 * c, row < it.rows ? 16 : 0);
             }
           }
-          if constexpr (C::kCodes) {
-            fence_proxy_async_smem();
-            mbar_arrive(bar(C::Q_FULL + qb));
-          } else {
-            cp_async_mbar_arrive_noinc(bar(C::Q_FULL + qb));
-          }
+          cp_async_mbar_arrive_noinc(bar((C::kCodes ? C::Q_RAW : C::Q_FULL) + qb));
           ++k;
         }
       }
@@ -908,6 +883,29 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         Item it;
         if (!next_item(k, it)) break;
         release_item(k);
+        // Q into the order of the converted K tiles, in place: after the item's first K, which the S
+        // MMAs need as early.
+        auto order_q = [&]() {
+          const int qb = k % C::kQBufs;
+          if (!waitw(bar(C::Q_RAW + qb), (uint32_t)(k / C::kQBufs) & 1u, ctl)) return false;
+          const uint32_t sq = sbase + (uint32_t)(C::kQ + qb * 2 * C::kTile);
+#pragma unroll 1
+          for (int x = 0; x < 2 * C::kTile / 16; x += 128 * 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[y] = lds128v(sq + (uint32_t)(x + 128 * y + ct) * 16u);
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              sts128(sq + (uint32_t)(x + 128 * y + ct) * 16u,
+                     make_uint4(__byte_perm(v[y].x, v[y].y, 0x5410), __byte_perm(v[y].x, v[y].y, 0x7632),
+                                __byte_perm(v[y].z, v[y].w, 0x5410), __byte_perm(v[y].z, v[y].w, 0x7632)));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::Q_FULL + qb));
+          return true;
+        };
+        if (it.c0 == it.c1) ok = order_q();
         for (int i = it.c0; i < it.c1 && ok; ++i, ++g) {
           const int kb = it.all.at(i) * kKeys, sl = g % C::kSlots;
 #pragma unroll 1
@@ -998,6 +996,10 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
             if (lane == 0) {
               mbar_arrive(bar((z ? C::V_OK : C::K_FULL) + sl));
               mbar_arrive(bar(C::CODE_EMPTY + cs));
+            }
+            if (z == 0 && i == it.c0 && !order_q()) {
+              ok = false;
+              break;
             }
           }
         }

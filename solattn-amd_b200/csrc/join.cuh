@@ -15,7 +15,7 @@ template <int D, int R, int T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int h, slot;
-  if (R == 16) {  // rows.cu
+  if (R <= 16) {  // rows.cu
     h = (int)(blockIdx.x % p.Hkv);
     slot = (int)(blockIdx.x / p.Hkv);
   } else {

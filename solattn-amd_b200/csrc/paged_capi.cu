@@ -8,7 +8,7 @@
 namespace solattn {
 
 cudaError_t launch_chunk(const SeqParams& p, int D, int kv, cudaStream_t stream);
-cudaError_t launch_rows(const SeqParams& p, int D, int kv, cudaStream_t stream);
+cudaError_t launch_rows(const SeqParams& p, int D, int kv, int rows, cudaStream_t stream);
 cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream);
 cudaError_t launch_cache_read(const CacheParams& p, int D, cudaStream_t stream);
 
@@ -40,26 +40,33 @@ bool rule_ok(const Rule& r) {
          r.sinks >= 0 && r.sinks < kNoBound;
 }
 
-// How the few-rows kernel divides a call: tiles of 16 rows (slots, see find_seq), and every tile's
-// keys over `splits` CTAs of at least `unit` 16-key chunks.
+// How a kernel divides a call: tiles of rows (slots, see find_seq), and a tile's keys over `splits` CTAs
+// of at least `unit` key tiles each.
 struct Split {
   int64_t slots, splits, unit;
-  int64_t first = 0;  // items before this one are not split
+  int64_t first = 0;  // chunk kernel: items before this one are not split
+  int64_t rows = 0;   // few-rows kernel: rows of a tile
 };
-Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t cap, bool paged,
-                 const Rule& r) {
+
+// The few-rows kernel: tiles of 8 rows where no sequence has more (half of the softmax of 16), 16 else;
+// units of 256 to 2048 keys, as many as give every SM some 8 CTAs, so that sequences of different
+// lengths even out.
+Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most, int64_t cap,
+                 bool paged, bool codes, const Rule& r) {
   Split s;
   const int64_t G = Hq / Hkv;
-  s.slots = paged && B > 1 ? N * G / 16 + B : B * cdiv((paged ? N : Tq) * G, 16);
+  s.rows = most <= 8 ? 8 : 16;
+  s.slots = paged && B > 1 ? N * G / s.rows + B : B * cdiv((paged ? N : Tq) * G, s.rows);
   int64_t keys = cap;
   if (r.window > 0 && r.lookahead >= 0) {
-    const int64_t span = r.window + r.lookahead + r.sinks + 16 + 48;
+    const int64_t span = r.window + r.lookahead + r.sinks + 16 + 64;
     if (span < keys) keys = span;
   }
-  const int64_t chunks = cdiv(keys, 16) + 2;
+  const int64_t chunk = D * (codes ? 1 : 2) >= 256 ? 16 : 32;  // keys of a chunk (rows.cu)
+  const int64_t chunks = cdiv(keys, chunk) + 2;
   int64_t unit = cdiv(chunks * s.slots * Hkv, kSms * 2 * 4);
-  if (unit < 16) unit = 16;
-  if (unit > 128) unit = 128;
+  if (unit < 256 / chunk) unit = 256 / chunk;
+  if (unit > 2048 / chunk) unit = 2048 / chunk;
   if (unit < cdiv(chunks, 64)) unit = cdiv(chunks, 64);
   s.unit = unit;
   s.splits = cdiv(chunks, unit);
@@ -118,16 +125,16 @@ struct Choice {
   int64_t rows_bytes, chunk_bytes;
 };
 Choice choose(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most_new, int64_t cap,
-              bool paged, const Rule& r) {
+              bool paged, bool codes, const Rule& r) {
   Choice c;
   const int64_t G = Hq / Hkv;
   const int64_t most = paged ? (most_new > 0 && most_new < N ? most_new : N) * G : Tq * G;
   const int64_t mean = paged ? N * G / B : Tq * G;
   c.many = most >= kManyRows;
   c.few = mean < kManyRows;
-  c.rows = rows_split(N, B, Hq, Hkv, Tq, cap, paged, r);
+  c.rows = rows_split(N, B, Hq, Hkv, D, Tq, c.many ? kManyRows : most, cap, paged, codes, r);
   c.chunk = chunk_split(N, B, Hq, Hkv, Tq, cap, paged, r);
-  c.rows_bytes = c.few ? split_bytes(c.rows, 16, Hkv, D) : 0;
+  c.rows_bytes = c.few ? split_bytes(c.rows, c.rows.rows, Hkv, D) : 0;
   c.chunk_bytes = c.many ? split_bytes(c.chunk, 256, Hkv, D) : 0;
   return c;
 }
@@ -184,7 +191,7 @@ int run(SeqParams& p, int64_t D, int kv, const Choice& c, void* workspace, int64
     x.max_new = !many && c.many ? (int)least - 1 : 0x7fffffff;
     x.zero_tail = p.zero_tail && !(many && c.few);
     const int rc = from_cuda(many ? launch_chunk(x, (int)D, kv, static_cast<cudaStream_t>(stream))
-                                  : launch_rows(x, (int)D, kv, static_cast<cudaStream_t>(stream)));
+                                  : launch_rows(x, (int)D, kv, (int)s.rows, static_cast<cudaStream_t>(stream)));
     if (rc) return rc;
   }
   return SOLATTN_OK;
@@ -223,7 +230,7 @@ int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_
                                        int64_t D, int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_window(B, Tq, Tk, Hq, Hkv, D, r)) return -1;
-  const Choice c = choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r);
+  const Choice c = choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, false, r);
   return c.rows_bytes + c.chunk_bytes;
 }
 
@@ -259,15 +266,15 @@ int solattn_window_attention(const void* q, const void* k, const void* v, int64_
   p.Tq = (int)Tq;
   p.Tk = (int)Tk;
   set_rule(p, r, scale);
-  return run(p, D, kStrided, choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r), workspace, workspace_bytes, stream);
+  return run(p, D, kStrided, choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, false, r), workspace, workspace_bytes, stream);
 }
 
 int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                                      int64_t page_size, int64_t table_width, int64_t most_new,
+                                      int codes, int64_t page_size, int64_t table_width, int64_t most_new,
                                       int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_paged(N, B, Hq, Hkv, D, page_size, table_width, r)) return -1;
-  const Choice c = choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r);
+  const Choice c = choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, codes != 0, r);
   return c.rows_bytes + c.chunk_bytes;
 }
 
@@ -312,7 +319,7 @@ int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, i
   p.zero_tail = zero_tail;
   set_rule(p, r, scale);
   return run(p, D, k_scale ? kPagedE4m3 : kPagedBf16,
-             choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r), workspace, workspace_bytes,
+             choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, k_scale != nullptr, r), workspace, workspace_bytes,
              stream);
 }
 
