@@ -360,9 +360,9 @@ SOLATTN_API int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, in
                       int64_t lookahead, int64_t sink_tokens, float scale, int zero_tail, void* workspace,
                       int64_t workspace_bytes, void* out, int32_t* status, void* stream);
 
-/* Workspace bytes of solattn_paged_attention (codes: E4M3 pages), or -1 on an invalid shape. */
+/* Workspace bytes of solattn_paged_attention, or -1 on an invalid shape. */
 SOLATTN_API int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                      int codes, int64_t page_size, int64_t table_width, int64_t most_new, int64_t window,
+                      int64_t page_size, int64_t table_width, int64_t most_new, int64_t window,
                       int64_t lookahead, int64_t sink_tokens);
 
 /*

@@ -52,7 +52,7 @@ struct Split {
 // units of 256 to 2048 keys, as many as give every SM some 8 CTAs, so that sequences of different
 // lengths even out.
 Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most, int64_t cap,
-                 bool paged, bool codes, const Rule& r) {
+                 bool paged, const Rule& r) {
   Split s;
   const int64_t G = Hq / Hkv;
   s.rows = most <= 8 ? 8 : 16;
@@ -62,7 +62,7 @@ Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
     const int64_t span = r.window + r.lookahead + r.sinks + 16 + 64;
     if (span < keys) keys = span;
   }
-  const int64_t chunk = D * (codes ? 1 : 2) >= 256 ? 16 : 32;  // keys of a chunk (rows.cu)
+  const int64_t chunk = D == 64 ? 32 : 16;  // keys of a chunk (rows.cu)
   const int64_t chunks = cdiv(keys, chunk) + 2;
   int64_t unit = cdiv(chunks * s.slots * Hkv, kSms * 2 * 4);
   if (unit < 256 / chunk) unit = 256 / chunk;
@@ -125,14 +125,14 @@ struct Choice {
   int64_t rows_bytes, chunk_bytes;
 };
 Choice choose(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most_new, int64_t cap,
-              bool paged, bool codes, const Rule& r) {
+              bool paged, const Rule& r) {
   Choice c;
   const int64_t G = Hq / Hkv;
   const int64_t most = paged ? (most_new > 0 && most_new < N ? most_new : N) * G : Tq * G;
   const int64_t mean = paged ? N * G / B : Tq * G;
   c.many = most >= kManyRows;
   c.few = mean < kManyRows;
-  c.rows = rows_split(N, B, Hq, Hkv, D, Tq, c.many ? kManyRows : most, cap, paged, codes, r);
+  c.rows = rows_split(N, B, Hq, Hkv, D, Tq, c.many ? kManyRows : most, cap, paged, r);
   c.chunk = chunk_split(N, B, Hq, Hkv, Tq, cap, paged, r);
   c.rows_bytes = c.few ? split_bytes(c.rows, c.rows.rows, Hkv, D) : 0;
   c.chunk_bytes = c.many ? split_bytes(c.chunk, 256, Hkv, D) : 0;
@@ -230,7 +230,7 @@ int64_t solattn_window_workspace_bytes(int64_t B, int64_t Tq, int64_t Tk, int64_
                                        int64_t D, int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_window(B, Tq, Tk, Hq, Hkv, D, r)) return -1;
-  const Choice c = choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, false, r);
+  const Choice c = choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r);
   return c.rows_bytes + c.chunk_bytes;
 }
 
@@ -266,15 +266,15 @@ int solattn_window_attention(const void* q, const void* k, const void* v, int64_
   p.Tq = (int)Tq;
   p.Tk = (int)Tk;
   set_rule(p, r, scale);
-  return run(p, D, kStrided, choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, false, r), workspace, workspace_bytes, stream);
+  return run(p, D, kStrided, choose(B * Tq, B, Hq, Hkv, D, Tq, 0, Tk, false, r), workspace, workspace_bytes, stream);
 }
 
 int64_t solattn_paged_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
-                                      int codes, int64_t page_size, int64_t table_width, int64_t most_new,
+                                      int64_t page_size, int64_t table_width, int64_t most_new,
                                       int64_t window, int64_t lookahead, int64_t sink_tokens) {
   const Rule r{window, lookahead, sink_tokens};
   if (check_paged(N, B, Hq, Hkv, D, page_size, table_width, r)) return -1;
-  const Choice c = choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, codes != 0, r);
+  const Choice c = choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r);
   return c.rows_bytes + c.chunk_bytes;
 }
 
@@ -319,7 +319,7 @@ int solattn_paged_attention(const void* q, int64_t N, int64_t Hq, int64_t Hkv, i
   p.zero_tail = zero_tail;
   set_rule(p, r, scale);
   return run(p, D, k_scale ? kPagedE4m3 : kPagedBf16,
-             choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, k_scale != nullptr, r), workspace, workspace_bytes,
+             choose(N, B, Hq, Hkv, D, 0, most_new, table_width * page_size, true, r), workspace, workspace_bytes,
              stream);
 }
 

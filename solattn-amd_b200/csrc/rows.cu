@@ -21,6 +21,7 @@ namespace solattn {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr float kTwo60 = 1152921504606846976.f, kTwoM60 = 1.f / kTwo60;
 constexpr int kRowThreads = kWarps * 32;
 
 // R rows of a tile: 8 or 16 (of the 16 rows of an MMA).  A chunk has 16 keys per MMA step, two steps
@@ -29,13 +30,15 @@ template <int D, int KV, int R>
 struct RowsCfg {
   static constexpr int kElt = KV == kPagedE4m3 ? 1 : 2;
   static constexpr int kRowB = D * kElt;          // bytes of a K or V row
-  static constexpr int kSteps = kRowB >= 256 ? 1 : 2;
+  static constexpr int kSteps = D == 64 ? 2 : 1;
   static constexpr int kChunk = 16 * kSteps;      // keys of a chunk
   static constexpr int kCpr = kRowB / 16;         // 16-byte pieces of a row
   static constexpr int kPart = kChunk * kRowB;    // K or V of a chunk
   static constexpr int kStage = 2 * kPart + (KV == kPagedE4m3 ? 2 * kChunk : 0);  // + K and V scales
-  // About 24 KB of ring per warp, so that two CTAs share an SM.
-  static constexpr int kStages = 24576 / kStage > 8 ? 8 : 24576 / kStage;
+  // BF16: 24 KB of ring per warp and two CTAs per SM (the bytes in flight are what counts); E4M3, which
+  // also has codes to convert: three or four CTAs, as many as the registers allow.
+  static constexpr int kStages = KV == kPagedE4m3 && D == 128 ? 4 : 3;
+  static constexpr int kCtas = KV != kPagedE4m3 ? 2 : D == 64 ? 4 : 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kMerge = kWarps * R * (D + 2) * 4;  // m, l, O of every warp
   static constexpr int kSmem = kWarps * kRing > kMerge ? kWarps * kRing : kMerge;
@@ -95,6 +98,23 @@ __device__ __forceinline__ float v_at(uint32_t sv, int key, int d) {
   return __uint_as_float((d & 1) ? (w & 0xffff0000u) : (w << 16));
 }
 
+// E4M3 codes 2 x and 2 x + 1 of a word as FP16, exactly (NaN stays NaN).
+__device__ __forceinline__ uint32_t codes_to_f16(uint32_t w, int x) {
+  uint32_t d;
+  const uint16_t two = (uint16_t)(x ? w >> 16 : w);
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(two));
+  return d;
+}
+
+// D = A(16x16 FP16, row) * B(16x8 FP16, col) + D, FP32 accumulate.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // Whether a pair of code fields (see e4m3_fields; signs cleared) is at E4M3's NaN: the largest pair so
 // far is kept, one instruction for two pairs.
 __device__ __forceinline__ bool nan_fields(uint32_t top) { return (top >> 16) == 0x7f0u || (top & 0xffffu) == 0x7f0u; }
@@ -129,12 +149,12 @@ __device__ __forceinline__ void exact_pv(float (&o)[D / 8][4], const float (&pr)
       p1 = __shfl_sync(0xffffffffu, p1, owner);
       s1 = __shfl_sync(0xffffffffu, (int)s1, owner) != 0;
     }
-    const float f = KV == kPagedE4m3 ? e8m0_value(lds8(scales + key)) : 1.f;
+    const float f = KV == kPagedE4m3 ? e8m0_value(lds8(scales + key)) * kTwoM60 : 1.f;
 #pragma unroll
     for (int nt = 0; nt < D / 8; ++nt) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float x = v_at<D, KV>(sv, key, out_dim<KV>(nt, t, c)) * f;
+        const float x = v_at<D, KV>(sv, key, out_dim<KV>(nt, t, c)) * f;  // (O holds 2^-60 of it, E4M3)
         if (s0) o[nt][c] += p0 * x;
         if (s1) o[nt][2 + c] += p1 * x;
       }
@@ -145,7 +165,7 @@ __device__ __forceinline__ void exact_pv(float (&o)[D / 8][4], const float (&pr)
 }  // namespace
 
 template <int D, int KV, int R>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
+__global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_kernel(const SeqParams p) {
   using C = RowsCfg<D, KV, R>;
   constexpr int kNt = 2 * C::kSteps;  // 8-key columns of a chunk
   extern __shared__ __align__(128) uint8_t smem[];
@@ -187,36 +207,43 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
   auto load = [&](int i) {
     const int key0 = C::kChunk * kt.at(c0 + warp + i * kWarps);
     const uint32_t st = ring + (uint32_t)((i % C::kStages) * C::kStage);
-    const bool whole = key0 + C::kChunk <= sq.L;  // else zeros behind the last key, which are not read
+    // Pieces of each 16-key step; rows behind the last key, and steps that nobody sees, become zeros
+    // without a read.
 #pragma unroll
     for (int u = 0; u < C::kSteps; ++u) {
+      const int key = key0 + 16 * u;
+      int page = 0;
+      if (KV != kStrided) page = __shfl_sync(0xffffffffu, my_page, (i % kAhead) * C::kSteps + u);
+      const int valid = page < 0 ? 0 : min(16, sq.L - key);
       const uint8_t *kp, *vp;
       int64_t kstep = C::kRowB, vstep = C::kRowB, row0 = 0;
-      bool there = true;
       if (KV == kStrided) {
-        kp = p.k + ((int64_t)sq.b * p.k_sB + (int64_t)(key0 + 16 * u) * p.k_sT + (int64_t)h * p.k_sH) * 2;
-        vp = p.v + ((int64_t)sq.b * p.v_sB + (int64_t)(key0 + 16 * u) * p.v_sT + (int64_t)h * p.v_sH) * 2;
+        kp = p.k + ((int64_t)sq.b * p.k_sB + (int64_t)key * p.k_sT + (int64_t)h * p.k_sH) * 2;
+        vp = p.v + ((int64_t)sq.b * p.v_sB + (int64_t)key * p.v_sT + (int64_t)h * p.v_sH) * 2;
         kstep = p.k_sT * 2;
         vstep = p.v_sT * 2;
-        there = key0 + 16 * u < sq.L;
-        if (!there) {
-          kp = p.k;
-          vp = p.v;
-        }
       } else {
-        const int page = __shfl_sync(0xffffffffu, my_page, (i % kAhead) * C::kSteps + u);
-        there = page >= 0;
-        row0 = (((int64_t)(there ? page : 0) * p.Hkv + h) << p.page_shift) + ((key0 + 16 * u) & ((1 << p.page_shift) - 1));
+        row0 = (((int64_t)max(page, 0) * p.Hkv + h) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
         kp = p.k + row0 * C::kRowB;
         vp = p.v + row0 * C::kRowB;
       }
+      kp += lr * kstep + 16 * lc;
+      vp += lr * vstep + 16 * lc;
+      const uint32_t dk = st + k_off<D, KV>(16 * u + lr, lc), dv = st + C::kPart;
+      if (valid == 16) {
 #pragma unroll
-      for (int j = 0; j < 16 / kPass; ++j) {
-        const int r = j * kPass + lr;
-        const bool in = there && (whole || key0 + 16 * u + r < sq.L);
-        const int64_t rr = in ? r : 0;
-        cp_async16(st + k_off<D, KV>(16 * u + r, lc), kp + rr * kstep + 16 * lc, in ? 16 : 0);
-        cp_async16(st + C::kPart + v_off<D, KV>(16 * u + r, lc), vp + rr * vstep + 16 * lc, in ? 16 : 0);
+        for (int j = 0; j < 16 / kPass; ++j) {
+          // (k_off only looks at r mod 2, which a pass keeps.)
+          cp_async16(dk + (uint32_t)(j * kPass * C::kRowB), kp + j * kPass * kstep, 16);
+          cp_async16(dv + v_off<D, KV>(16 * u + j * kPass + lr, lc), vp + j * kPass * vstep, 16);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16 / kPass; ++j) {
+          const bool in = j * kPass + lr < valid;
+          cp_async16(dk + (uint32_t)(j * kPass * C::kRowB), in ? kp + j * kPass * kstep : p.k, in ? 16 : 0);
+          cp_async16(dv + v_off<D, KV>(16 * u + j * kPass + lr, lc), in ? vp + j * kPass * vstep : p.v, in ? 16 : 0);
+        }
       }
       if (KV == kPagedE4m3 && lane < 2)
         cp_async16(st + 2 * C::kPart + C::kChunk * lane + 16 * u, (lane ? p.v_scale : p.k_scale) + row0, 16);
@@ -230,11 +257,14 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
   }
 
   // Q fragments: the contraction order over the head dim is free, so lane t of a row group holds the
-  // dims that its 16-byte K reads deliver: k-step ks takes 4 consecutive dims of piece 4 (ks / S) + t
-  // (E4M3: in the order 0, 2, 1, 3, in which a word of codes falls apart without byte moves).
+  // dims that its 16-byte K reads deliver: k-step ks takes 4 consecutive dims of piece 4 (ks / S) + t.
+  // E4M3: S on FP16, in which codes are exact and cheap to make.  A row of Q is scaled by a power of two
+  // that puts its largest value below 2^15; BF16's 8 significant bits fit in FP16's 11, and what falls
+  // below FP16's range is 2^-39 of that value.
   constexpr int kS = C::kElt == 1 ? 4 : 2;  // k-steps of a 16-byte piece
   uint32_t qa[D / 16][4];
   int hi[C::kHalves], lo[C::kHalves];  // what rows g and g + 8 see
+  float qf[C::kHalves];                // S in log2 units = qf * (Q K^T)
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = g + 8 * half;
@@ -248,10 +278,35 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
       const int d = (16 / C::kElt) * (4 * (ks / kS) + t) + 4 * (ks % kS);
       uint2 w = make_uint2(0u, 0u);
       if (half < C::kHalves && in) w = __ldg(reinterpret_cast<const uint2*>(src + d));
-      qa[ks][half] = KV == kPagedE4m3 ? __byte_perm(w.x, w.y, 0x5410) : w.x;
-      qa[ks][2 + half] = KV == kPagedE4m3 ? __byte_perm(w.x, w.y, 0x7632) : w.y;
+      qa[ks][half] = w.x;
+      qa[ks][2 + half] = w.y;
     }
     if (half < C::kHalves) {
+      qf[half] = p.scale_log2;
+      if (KV == kPagedE4m3) {
+        float top = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t w = qa[ks][2 * x + half];
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w << 16)), fabsf(__uint_as_float(w & 0xffff0000u))));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // top < 2^(e + 1): Q * 2^(14 - e) < 2^15.
+        const int e = min(127, max(-100, (int)(__float_as_uint(top) >> 23) - 127));
+        const float f = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+        qf[half] *= __uint_as_float((uint32_t)(127 - 14 + e) << 23);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t w = qa[ks][2 * x + half];
+            const __half2 y = __floats2half2_rn(__uint_as_float(w << 16) * f, __uint_as_float(w & 0xffff0000u) * f);
+            qa[ks][2 * x + half] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+      }
       const int pos = off + (r_base + r) / p.G;
       hi[half] = in ? key_high(p, sq.L, pos) : -1;
       lo[half] = key_low(p, pos);
@@ -285,12 +340,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
 
     // ---- S = Q K^T: 16 rows, tiles of 8 keys
     float s[kNt][4];
-    uint32_t k_top[kNt];  // E4M3: the largest code fields in this lane's part of key 8 nt + g
 #pragma unroll
-    for (int nt = 0; nt < kNt; ++nt) {
-      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-      k_top[nt] = 0u;
-    }
+    for (int nt = 0; nt < kNt; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
     for (int hh = 0; hh < C::kCpr / 4; ++hh) {
 #pragma unroll
@@ -299,13 +350,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
         if (KV == kPagedE4m3) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t odd = (w[x] >> 4) & 0x07f007f0u, even = (w[x] << 4) & 0x07f007f0u;
-            k_top[nt] = __vimax3_u16x2(k_top[nt], odd, even);
-            const uint32_t b0 = bf16x2_mul(even | ((w[x] << 8) & 0x80008000u), kTwo120x2);
-            const uint32_t b1 = bf16x2_mul(odd | (w[x] & 0x80008000u), kTwo120x2);
-            mma_bf16_16816(s[nt], qa[4 * hh + x], b0, b1);
-          }
+          for (int x = 0; x < 4; ++x)
+            mma_f16_16816(s[nt], qa[4 * hh + x], codes_to_f16(w[x], 0), codes_to_f16(w[x], 1));
         } else {
           mma_bf16_16816(s[nt], qa[2 * hh], w[0], w[1]);
           mma_bf16_16816(s[nt], qa[2 * hh + 1], w[2], w[3]);
@@ -314,12 +360,12 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
     }
     // Scales: lane l converts those of key l, then each lane takes its columns' (keys 8 nt + 2 t + c).
     float vs[kNt][2];
-    bool scale_nan = false;
+    bool odd_scale = false;
     if (KV == kPagedE4m3) {
       const int key = lane & (C::kChunk - 1);
-      const float ks_l = e8m0_value(lds8(st + 2 * C::kPart + key)) * p.scale_log2;
+      const float ks_l = e8m0_value(lds8(st + 2 * C::kPart + key));
       const float vs_l = e8m0_value(lds8(st + 2 * C::kPart + C::kChunk + key));
-      scale_nan = vs_l != vs_l;
+      odd_scale = !(vs_l < kTwo60 / 2);  // (or one that P cannot take, see below)
 #pragma unroll
       for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
@@ -329,30 +375,9 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half) s[nt][2 * half + c] *= f;
         }
-      bool k_nan = false;
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) k_nan = k_nan || nan_fields(k_top[nt]);
-      if (__any_sync(0xffffffffu, k_nan)) {  // (rare) a NaN code in K: the key's scores are NaN
-        uint32_t flags = 0u;
-#pragma unroll
-        for (int nt = 0; nt < kNt; ++nt) flags |= nan_fields(k_top[nt]) ? 1u << nt : 0u;
-        flags |= __shfl_xor_sync(0xffffffffu, flags, 1);
-        flags |= __shfl_xor_sync(0xffffffffu, flags, 2);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t f = __shfl_sync(0xffffffffu, flags, 4 * (2 * t + c));  // of keys 8 nt + 2 t + c
-#pragma unroll
-          for (int nt = 0; nt < kNt; ++nt)
-            if ((f >> nt) & 1u) s[nt][c] = s[nt][2 + c] = __uint_as_float(0x7fc00000u);
-        }
-      }
     } else {
 #pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) {
-#pragma unroll
-        for (int c = 0; c < 2 * C::kHalves; ++c) s[nt][c] *= p.scale_log2;
-        vs[nt][0] = vs[nt][1] = 1.f;
-      }
+      for (int nt = 0; nt < kNt; ++nt) vs[nt][0] = vs[nt][1] = 1.f;
     }
     // ---- visibility
     bool vis[kNt][4];
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
 #pragma unroll
       for (int nt = 1; nt < kNt; ++nt) x = fmaxf(x, fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * qf[half];
       if (m[half] == -INFINITY) {
         m[half] = fmaxf(m[half], x);  // nothing accumulated yet
       } else if (x > m[half] + 8.f) {
@@ -409,13 +434,20 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
       for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          pr[nt][2 * half + c] = fast_exp2(s[nt][2 * half + c] - mm);
+          pr[nt][2 * half + c] = fast_exp2(fmaf(s[nt][2 * half + c], qf[half], -mm));
           l[half] += pr[nt][2 * half + c];
         }
     }
     // P as the A operand: rounded to BF16 (relative error at most 2^-8 each; l keeps FP32), E4M3 with
-    // V's power-of-two scale folded in, which rounds the same.
+    // V's power-of-two scale folded in, which rounds the same, and 2^60 of the 2^120 that V's code
+    // fields lack (O takes the rest at the end; the products then lie well inside FP32's range).
     uint32_t pa[C::kSteps][4];
+    if (KV == kPagedE4m3) {
+#pragma unroll
+      for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) vs[nt][c] *= kTwo60;
+    }
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt) {
       pa[nt >> 1][2 * (nt & 1)] = pack_bf16(pr[nt][0] * vs[nt][0], pr[nt][1] * vs[nt][1]);
@@ -444,11 +476,11 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
             const uint32_t a = __byte_perm(w[0], w[1], sel), b = __byte_perm(w[2], w[3], sel);
             const uint32_t fa = (a >> 4) & 0x07f007f0u, fb = (b >> 4) & 0x07f007f0u;
             top = __vimax3_u16x2(top, fa, fb);
-            vb[u][4 * j + x][0] = bf16x2_mul(fa | (a & 0x80008000u), kTwo120x2);
-            vb[u][4 * j + x][1] = bf16x2_mul(fb | (b & 0x80008000u), kTwo120x2);
+            vb[u][4 * j + x][0] = fa | (a & 0x80008000u);
+            vb[u][4 * j + x][1] = fb | (b & 0x80008000u);
           }
         }
-      bad = nan_fields(top) || scale_nan;
+      bad = nan_fields(top) || odd_scale;
     } else {
       uint32_t acc = 0u;  // V * 0 summed: NaN where a V is not finite
 #pragma unroll
@@ -490,7 +522,8 @@ __global__ void __launch_bounds__(kRowThreads) rows_kernel(const SeqParams p) {
 #pragma unroll
       for (int nt = 0; nt < D / 8; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) dst[out_dim<KV>(nt, t, c)] = o[nt][2 * half + c];
+        for (int c = 0; c < 2; ++c)
+          dst[out_dim<KV>(nt, t, c)] = KV == kPagedE4m3 ? o[nt][2 * half + c] * kTwo60 : o[nt][2 * half + c];
       if (t == 0) {
         sM[(warp * R + r) * 2] = m[half];
         sM[(warp * R + r) * 2 + 1] = l[half];
@@ -542,7 +575,7 @@ namespace {
 template <int D, int KV, int R>
 cudaError_t launch_rows_kv(const SeqParams& p, cudaStream_t stream) {
   using C = RowsCfg<D, KV, R>;
-  static_assert(C::kSmem <= 113 * 1024, "two CTAs share an SM");
+  static_assert(C::kCtas * (C::kSmem + 1024) <= 227 * 1024, "CTAs that share an SM");
   cudaError_t err = cudaFuncSetAttribute(rows_kernel<D, KV, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (err != cudaSuccess) return err;
   const int64_t tiles = (int64_t)p.slots * p.Hkv;

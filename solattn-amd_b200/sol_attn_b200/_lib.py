@@ -55,7 +55,7 @@ SIGNATURES = {
     "solattn_window_workspace_bytes": (_I64, [_I64] * 9),
     "solattn_paged_attention": (c_int, [_P] + [_I64] * 6 + [_P] * 4 + [_I64] * 2 + [_P, _I64, _P, _P]
                                 + [_I64] * 5 + [c_float, c_int, _P, _I64, _P, _P, _P]),
-    "solattn_paged_workspace_bytes": (_I64, [_I64] * 5 + [c_int] + [_I64] * 6),
+    "solattn_paged_workspace_bytes": (_I64, [_I64] * 11),
     "solattn_cache_write": (c_int, [_P, _P] + [_I64] * 7 + [_P] * 4 + [_I64] * 2
                             + [_P, _I64, _P, _P, _I64, _P, _P]),
     "solattn_cache_read": (c_int, [_P] * 4 + [_I64] * 2 + [_P, _I64, _P] + [_I64] * 4 + [_P] * 4),

@@ -252,8 +252,7 @@ def _attend(q, cache, plan, rule, scale, out):
     fresh = out is None
     word = monitor(q.device).word()
     keep, ws, size = workspace("solattn_paged_workspace_bytes",
-                               (N, B, Hq, cache.heads, D, int(cache.k_scale is not None), cache.page_size, width,
-                                plan.most_new, *rule), q.device)
+                               (N, B, Hq, cache.heads, D, cache.page_size, width, plan.most_new, *rule), q.device)
     if fresh:
         out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
     rc = _lib.load().solattn_paged_attention(
