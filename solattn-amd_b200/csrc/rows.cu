@@ -21,7 +21,8 @@ namespace solattn {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr float kTwo60 = 1152921504606846976.f, kTwoM60 = 1.f / kTwo60;
+constexpr int kScaleRoom = 13;  // E4M3: P * 2^13 fits in FP16 (P is at most 4)
+constexpr int kScaleSpan = 12;  // and may be 2^12 smaller for a key with a smaller V scale
 constexpr int kRowThreads = kWarps * 32;
 
 // R rows of a tile: 8 or 16 (of the 16 rows of an MMA).  A chunk has 16 keys per MMA step, two steps
@@ -47,7 +48,7 @@ struct RowsCfg {
 
 // Shared-memory offsets of the 16-byte piece c of row r, chosen so that the reads below have no bank
 // conflicts: K is read as 16 bytes by lane (row = lane / 4, piece = 4 i + lane % 4); BF16 V by
-// ldmatrix (8 rows, one piece); E4M3 V as 4 bytes (rows 2 t, t = lane % 4; 32 bytes by lane / 4).
+// ldmatrix (8 rows, one piece), of 8-bit elements for E4M3.
 template <int D, int KV>
 __device__ __forceinline__ uint32_t k_off(int r, int c) {
   constexpr int kRowB = KV == kPagedE4m3 ? D : 2 * D;
@@ -56,10 +57,7 @@ __device__ __forceinline__ uint32_t k_off(int r, int c) {
 template <int D, int KV>
 __device__ __forceinline__ uint32_t v_off(int r, int c) {
   constexpr int kRowB = KV == kPagedE4m3 ? D : 2 * D;
-  if (KV != kPagedE4m3) return (uint32_t)(r * kRowB + ((c ^ (r & 7)) << 4));
-  if (D == 128) return (uint32_t)(r * kRowB + ((c ^ (((r >> 1) & 3) << 1)) << 4));
-  const int phys = (r & ~3) | ((r & 1) << 1) | ((r >> 1) & 1);
-  return (uint32_t)(phys * kRowB + ((c ^ (((r >> 2) & 1) << 1)) << 4));
+  return (uint32_t)(r * kRowB + ((c ^ (kRowB >= 128 ? r & 7 : (r >> 1) & 3)) << 4));
 }
 
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -80,13 +78,26 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
   return v;
 }
 
-// The head dim of column `col` (0 or 1) of this lane's pair in output tile nt (8 columns).  BF16: the
-// tile's own.  E4M3: a lane's 4-byte read covers four tiles' columns, so that tile (4 j + i) holds the
-// dims 32 j + 4 g + i, g = 0..7.
+// The key (within a chunk) of column 2 t + c of the 8-key tile nt.  E4M3: a transposed read of V gives a
+// lane 4 consecutive keys of a head dim, so the keys of a 16-key step are dealt out to match.
 template <int KV>
-__device__ __forceinline__ int out_dim(int nt, int t, int col) {
-  return KV == kPagedE4m3 ? 32 * (nt >> 2) + 8 * t + 4 * col + (nt & 3) : 8 * nt + 2 * t + col;
+__device__ __forceinline__ int key_of(int nt, int t, int c) {
+  return KV == kPagedE4m3 ? 16 * (nt >> 1) + 4 * t + 2 * (nt & 1) + c : 8 * nt + 2 * t + c;
 }
+
+// 16 x 16 codes twice, transposed: lane l gets keys 4 (l % 4) .. + 3 of dim l / 4 (and + 8) of each.
+__device__ __forceinline__ void ldsm_codes_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// 2^e, zero where that is below FP32's normal range (e at most 127).
+__device__ __forceinline__ float two_to(int e) { return e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23); }
 
 template <int D, int KV>
 __device__ __forceinline__ float v_at(uint32_t sv, int key, int d) {
@@ -115,27 +126,26 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Whether a pair of code fields (see e4m3_fields; signs cleared) is at E4M3's NaN: the largest pair so
-// far is kept, one instruction for two pairs.
-__device__ __forceinline__ bool nan_fields(uint32_t top) { return (top >> 16) == 0x7f0u || (top & 0xffffu) == 0x7f0u; }
-
-// O += P V of one chunk with a non-finite V, key by key and only where the row sees the key.
-// `scales` is the chunk's V exponents (E4M3).
+// O += P V of one chunk whose V is not finite (or, E4M3, whose scales lie too far apart), key by key and
+// only where the row sees the key.  `scales` is the chunk's V exponents, O holds 2^(127 + 13 - ref) of
+// its value (E4M3).
 template <int D, int KV, int R>
 __device__ __forceinline__ void exact_pv(float (&o)[D / 8][4], const float (&pr)[2 * RowsCfg<D, KV, R>::kSteps][4],
                                          const bool (&vis)[2 * RowsCfg<D, KV, R>::kSteps][4], uint32_t sv,
-                                         uint32_t scales, int lane) {
+                                         uint32_t scales, int ref, int lane) {
   const int t = lane & 3;
 #pragma unroll 1
   for (int key = 0; key < RowsCfg<D, KV, R>::kChunk; ++key) {
-    const int owner = (lane & ~3) | ((key & 7) >> 1);
+    // Tile, lane and column of the key (key_of backwards).
+    const int tile = KV == kPagedE4m3 ? 2 * (key >> 4) + ((key >> 1) & 1) : key >> 3;
+    const int owner = (lane & ~3) | (KV == kPagedE4m3 ? (key & 15) >> 2 : (key & 7) >> 1);
     float p0 = 0.f, p1 = 0.f;
     bool s0 = false, s1 = false;
 #pragma unroll
     for (int nt = 0; nt < 2 * RowsCfg<D, KV, R>::kSteps; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        if ((key >> 3) == nt && (key & 1) == c) {
+        if (tile == nt && (key & 1) == c) {
           p0 = pr[nt][c];
           s0 = vis[nt][c];
           if (R == 16) {
@@ -149,12 +159,16 @@ __device__ __forceinline__ void exact_pv(float (&o)[D / 8][4], const float (&pr)
       p1 = __shfl_sync(0xffffffffu, p1, owner);
       s1 = __shfl_sync(0xffffffffu, (int)s1, owner) != 0;
     }
-    const float f = KV == kPagedE4m3 ? e8m0_value(lds8(scales + key)) * kTwoM60 : 1.f;
+    float f = 1.f;
+    if (KV == kPagedE4m3) {
+      const int e = (int)lds8(scales + key);
+      f = e == 255 ? __uint_as_float(0x7fc00000u) : two_to(min(127, e - ref + kScaleRoom));
+    }
 #pragma unroll
     for (int nt = 0; nt < D / 8; ++nt) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float x = v_at<D, KV>(sv, key, out_dim<KV>(nt, t, c)) * f;  // (O holds 2^-60 of it, E4M3)
+        const float x = v_at<D, KV>(sv, key, 8 * nt + 2 * t + c) * f;
         if (s0) o[nt][c] += p0 * x;
         if (s1) o[nt][2 + c] += p1 * x;
       }
@@ -324,6 +338,8 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
     l[half] = 0.f;
   }
 
+  int ref = 0;  // E4M3: O's scale, as an E8M0 exponent
+
 #pragma unroll 1
   for (int i = 0; i < mine; ++i) {
     cp_async_wait<C::kStages - 2>();
@@ -346,7 +362,7 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
     for (int hh = 0; hh < C::kCpr / 4; ++hh) {
 #pragma unroll
       for (int nt = 0; nt < kNt; ++nt) {
-        const uint4 w4 = lds128(st + k_off<D, KV>(8 * nt + g, 4 * hh + t));
+        const uint4 w4 = lds128(st + k_off<D, KV>(key_of<KV>(nt, g >> 1, g & 1), 4 * hh + t));
         const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
         if (KV == kPagedE4m3) {
 #pragma unroll
@@ -358,30 +374,46 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
         }
       }
     }
-    // Scales: lane l converts those of key l, then each lane takes its columns' (keys 8 nt + 2 t + c).
+    const bool full = key0 + C::kChunk - 1 <= all_hi && (key0 >= all_lo || key0 + C::kChunk <= p.sinks);
+    // E4M3 scales: lane l has those of key l; each lane takes its columns'.  P V runs on FP16 too: P is
+    // multiplied by 2^13 and by the key's V scale relative to `ref`, the largest scale seen so far, to
+    // which O is relative as well.  FP16 then holds every P that matters (down to 2^-37 of the largest
+    // for keys at `ref`, 2^-25 for keys 2^12 below); a chunk with a scale that is further below, or NaN,
+    // goes through exact_pv.  Scales of keys that nobody sees do not count, nor do those of 2^-127
+    // (rows of zeros, or of values below 2^-118).
     float vs[kNt][2];
     bool odd_scale = false;
     if (KV == kPagedE4m3) {
       const int key = lane & (C::kChunk - 1);
       const float ks_l = e8m0_value(lds8(st + 2 * C::kPart + key));
-      const float vs_l = e8m0_value(lds8(st + 2 * C::kPart + C::kChunk + key));
-      odd_scale = !(vs_l < kTwo60 / 2);  // (or one that P cannot take, see below)
+      int e = (int)lds8(st + 2 * C::kPart + C::kChunk + key);
+      if (!full && (key0 + key > high || (key0 + key < low && key0 + key >= p.sinks))) e = 0;
+      odd_scale = __any_sync(0xffffffffu, e == 255);
+      if (e == 255) e = 0;
+      const int most = __reduce_max_sync(0xffffffffu, e);
+      const int least = __reduce_min_sync(0xffffffffu, e == 0 ? 255 : e);
+      if (most > ref) {
+        const float f = two_to(ref - most);
+        ref = most;
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[x][c] *= f;
+      }
+      odd_scale = odd_scale || least < ref - kScaleSpan;
+      const float vs_l = e == 0 ? 0.f : two_to(e - ref + kScaleRoom);
 #pragma unroll
       for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const float f = __shfl_sync(0xffffffffu, ks_l, 8 * nt + 2 * t + c);
-          vs[nt][c] = __shfl_sync(0xffffffffu, vs_l, 8 * nt + 2 * t + c);
+          const float f = __shfl_sync(0xffffffffu, ks_l, key_of<KV>(nt, t, c));
+          vs[nt][c] = __shfl_sync(0xffffffffu, vs_l, key_of<KV>(nt, t, c));
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half) s[nt][2 * half + c] *= f;
         }
-    } else {
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) vs[nt][0] = vs[nt][1] = 1.f;
     }
     // ---- visibility
     bool vis[kNt][4];
-    const bool full = key0 + C::kChunk - 1 <= all_hi && (key0 >= all_lo || key0 + C::kChunk <= p.sinks);
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
@@ -391,13 +423,13 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
       for (int nt = 0; nt < kNt; ++nt)
 #pragma unroll
         for (int c = 0; c < 2 * C::kHalves; ++c) {
-          const int key = key0 + 8 * nt + 2 * t + (c & 1), half = c >> 1;
+          const int key = key0 + key_of<KV>(nt, t, c & 1), half = c >> 1;
           vis[nt][c] = key <= hi[half] && (key >= lo[half] || key < p.sinks);
           if (!vis[nt][c]) s[nt][c] = -INFINITY;
         }
     }
     // ---- online softmax.  The running maximum moves only when it grows by more than 8 (a factor
-    // 256), so that O is rarely rescaled; P stays at most 256.
+    // 256), so that O is rarely rescaled; P stays at most 256.  (E4M3: 2, for FP16's sake.)
     float al[2] = {1.f, 1.f};
     bool need = false;
 #pragma unroll
@@ -409,7 +441,7 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
       x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * qf[half];
       if (m[half] == -INFINITY) {
         m[half] = fmaxf(m[half], x);  // nothing accumulated yet
-      } else if (x > m[half] + 8.f) {
+      } else if (x > m[half] + (KV == kPagedE4m3 ? 2.f : 8.f)) {
         al[half] = fast_exp2(m[half] - x);
         m[half] = x;
         need = true;
@@ -438,53 +470,39 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
           l[half] += pr[nt][2 * half + c];
         }
     }
-    // P as the A operand: rounded to BF16 (relative error at most 2^-8 each; l keeps FP32), E4M3 with
-    // V's power-of-two scale folded in, which rounds the same, and 2^60 of the 2^120 that V's code
-    // fields lack (O takes the rest at the end; the products then lie well inside FP32's range).
+    // P as the A operand: rounded to BF16 (relative error at most 2^-8 each; l keeps FP32), or, with its
+    // scale, to FP16 (2^-11).
     uint32_t pa[C::kSteps][4];
-    if (KV == kPagedE4m3) {
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) vs[nt][c] *= kTwo60;
-    }
+    auto pack = [&](float a, float b) {
+      if (KV != kPagedE4m3) return pack_bf16(a, b);
+      const __half2 y = __floats2half2_rn(a, b);
+      return *reinterpret_cast<const uint32_t*>(&y);
+    };
 #pragma unroll
     for (int nt = 0; nt < kNt; ++nt) {
-      pa[nt >> 1][2 * (nt & 1)] = pack_bf16(pr[nt][0] * vs[nt][0], pr[nt][1] * vs[nt][1]);
-      pa[nt >> 1][2 * (nt & 1) + 1] =
-          R == 16 ? pack_bf16(pr[nt][2] * vs[nt][0], pr[nt][3] * vs[nt][1]) : 0u;
+      const float f0 = KV == kPagedE4m3 ? vs[nt][0] : 1.f, f1 = KV == kPagedE4m3 ? vs[nt][1] : 1.f;
+      pa[nt >> 1][2 * (nt & 1)] = pack(pr[nt][0] * f0, pr[nt][1] * f1);
+      pa[nt >> 1][2 * (nt & 1) + 1] = R == 16 ? pack(pr[nt][2] * f0, pr[nt][3] * f1) : 0u;
     }
-    // ---- O += P V, once V is known to be finite
+    // ---- O += P V, once V is known to be finite (V * 0 summed is NaN where it is not)
     uint32_t vb[C::kSteps][D / 8][2];
-    bool bad = false;
-    if (KV == kPagedE4m3) {
-      uint32_t top = 0u;
+    uint32_t acc = 0u;
 #pragma unroll
-      for (int u = 0; u < C::kSteps; ++u)
+    for (int u = 0; u < C::kSteps; ++u) {
+      if (KV == kPagedE4m3) {
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t w[4];  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of the step; dims 32 j + 4 g..
+        for (int dd = 0; dd < D / 32; ++dd) {
+          uint32_t w[4];
+          ldsm_codes_t(sv + v_off<D, KV>(16 * u + (lane & 15), 2 * dd + (lane >> 4)), w);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int key = 16 * u + 2 * t + (x & 1) + 8 * (x >> 1);
-            w[x] = lds32(sv + v_off<D, KV>(key, 2 * j + (g >> 2)) + (uint32_t)(4 * (g & 3)));
-          }
+          for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            // Byte x of two keys' words into the high bytes of a pair; the fields mask drops the rest.
-            const uint32_t sel = (uint32_t)(x << 4) | (uint32_t)((4 + x) << 12);
-            const uint32_t a = __byte_perm(w[0], w[1], sel), b = __byte_perm(w[2], w[3], sel);
-            const uint32_t fa = (a >> 4) & 0x07f007f0u, fb = (b >> 4) & 0x07f007f0u;
-            top = __vimax3_u16x2(top, fa, fb);
-            vb[u][4 * j + x][0] = fa | (a & 0x80008000u);
-            vb[u][4 * j + x][1] = fb | (b & 0x80008000u);
-          }
+            for (int y = 0; y < 2; ++y) {
+              vb[u][4 * dd + x][y] = codes_to_f16(w[x], y);
+              acc = f16x2_fma(vb[u][4 * dd + x][y], 0u, acc);
+            }
         }
-      bad = nan_fields(top) || odd_scale;
-    } else {
-      uint32_t acc = 0u;  // V * 0 summed: NaN where a V is not finite
-#pragma unroll
-      for (int u = 0; u < C::kSteps; ++u)
+      } else {
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) {
           ldsm_x4_t(sv + v_off<D, KV>(16 * u + (lane & 15), 2 * dt + (lane >> 4)), vb[u][2 * dt][0],
@@ -495,15 +513,19 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
             acc = bf16x2_fma(vb[u][2 * dt + x][1], 0u, acc);
           }
         }
-      bad = (acc & 0x7fff7fffu) != 0u;
+      }
     }
+    const bool bad = (acc & 0x7fff7fffu) != 0u || odd_scale;
     if (__any_sync(0xffffffffu, bad)) {
-      exact_pv<D, KV, R>(o, pr, vis, sv, st + 2 * C::kPart + C::kChunk, lane);
+      exact_pv<D, KV, R>(o, pr, vis, sv, st + 2 * C::kPart + C::kChunk, ref, lane);
     } else {
 #pragma unroll
       for (int u = 0; u < C::kSteps; ++u)
 #pragma unroll
-        for (int nt = 0; nt < D / 8; ++nt) mma_bf16_16816(o[nt], pa[u], vb[u][nt][0], vb[u][nt][1]);
+        for (int nt = 0; nt < D / 8; ++nt) {
+          if (KV == kPagedE4m3) mma_f16_16816(o[nt], pa[u], vb[u][nt][0], vb[u][nt][1]);
+          else mma_bf16_16816(o[nt], pa[u], vb[u][nt][0], vb[u][nt][1]);
+        }
     }
   }
   cp_async_wait<0>();
@@ -523,7 +545,8 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
       for (int nt = 0; nt < D / 8; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          dst[out_dim<KV>(nt, t, c)] = KV == kPagedE4m3 ? o[nt][2 * half + c] * kTwo60 : o[nt][2 * half + c];
+          dst[8 * nt + 2 * t + c] = KV == kPagedE4m3 ? o[nt][2 * half + c] * two_to(-kScaleRoom) * e8m0_value((uint32_t)ref)
+                                                     : o[nt][2 * half + c];
       if (t == 0) {
         sM[(warp * R + r) * 2] = m[half];
         sM[(warp * R + r) * 2 + 1] = l[half];

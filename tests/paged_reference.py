@@ -84,12 +84,15 @@ def values(codes, scales):
 class Sequences:
     """A paged cache with random K/V for sequences of the given (new, keys), pages in random order."""
 
-    def __init__(self, counts, *, heads, dim, page, kind, seed=0, extra=2, device="cuda", width=None):
+    def __init__(self, counts, *, heads, dim, page, kind, seed=0, extra=2, device="cuda", width=None,
+                 v_gain=None):
         from sol_attn_b200 import PagedKVCache, PagedPlan
         gen = torch.Generator().manual_seed(seed)
         self.counts, self.page = counts, page
         self.k = [torch.randn((L, heads, dim), generator=gen, dtype=torch.bfloat16) * 2 for _, L in counts]
         self.v = [torch.randn((L, heads, dim), generator=gen, dtype=torch.bfloat16) for _, L in counts]
+        if v_gain is not None:  # (L, heads) -> factors of V's rows
+            self.v = [x * v_gain(*x.shape[:2])[..., None].to(x.dtype) for x in self.v]
         used = [-(-L // page) for _, L in counts]
         pages = sum(used) + extra
         order = torch.randperm(pages, generator=gen)

@@ -156,6 +156,37 @@ def test_e4m3_nan_codes_and_scales(new):
     check_device_errors()
 
 
+@pytest.mark.parametrize("new", [1, 3, 150])
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("spread", [6, 40])
+def test_e4m3_scales_far_apart(new, D, page, spread):
+    """V rows (and so their scales) that differ by powers of two, rows of zeros among them, large ones
+    that only a few queries see, and one so large that it dwarfs the rest."""
+    gen = torch.Generator().manual_seed(11)
+
+    def gain(L, heads):
+        g = torch.exp2(torch.randint(-spread, 4, (L, heads), generator=gen).float())
+        g[::7] = 0
+        g[L // 2] = 2.0 ** 30
+        return g
+
+    s = Sequences([(new, 500), (1, 33)], heads=2, dim=D, page=page, kind="e4m3", v_gain=gain)
+    q = s.queries(4, D)
+    for rule in (dict(), dict(window=100, sink_tokens=5)):
+        assert_within(paged_attention(q.cuda(), s.cache, s.plan, **rule), *s.expected(q, **rule))
+    check_device_errors()
+
+
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_large_scores(kind, new):
+    """Scores of hundreds, at which the running maximum moves in most tiles."""
+    s = Sequences([(new, 700)], heads=1, dim=64, page=16, kind=kind)
+    q = s.queries(2, 64) * 40
+    assert_within(paged_attention(q.cuda(), s.cache, s.plan), *s.expected(q))
+    check_device_errors()
+
+
 def test_pages_that_no_key_needs_are_not_read():
     """Window pages given back (-1, or far outside) are never addressed; a needed one is reported."""
     s = Sequences([(1, 640)], heads=1, dim=64, page=16, kind="bf16")
