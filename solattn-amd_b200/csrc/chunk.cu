@@ -250,6 +250,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
   uint32_t* redo = reinterpret_cast<uint32_t*>(smem + C::kRedo);
   const Ctl ctl{reinterpret_cast<volatile int*>(misc + 1), p.status};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_trigger();
 
   if (tid == 0) {
     for (int i = 0; i < C::NBARS; ++i) {
@@ -1048,11 +1049,17 @@ cudaError_t launch_chunk_kv(const SeqParams& p, cudaStream_t stream) {
   if (KV == kPagedBf16 && (!paged_map(&tmK, p.k, p, D) || !paged_map(&tmV, p.v, p, D))) return cudaErrorInvalidValue;
   auto* kernel = chunk_kernel<D, KV>;
   // setmaxnreg divides exactly the registers that the launch holds: with fewer it would wait for good.
-  cudaFuncAttributes attr;
-  cudaError_t err = cudaFuncGetAttributes(&attr, kernel);
-  if (err != cudaSuccess) return err;
-  if (attr.numRegs != C::kLaunchRegs) return cudaErrorInvalidDeviceFunction;
-  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes);
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> regs{0};
+  cudaError_t err;
+  if (regs.load(std::memory_order_relaxed) == 0) {
+    cudaFuncAttributes attr;
+    err = cudaFuncGetAttributes(&attr, kernel);
+    if (err != cudaSuccess) return err;
+    regs.store(attr.numRegs, std::memory_order_relaxed);
+  }
+  if (regs.load(std::memory_order_relaxed) != C::kLaunchRegs) return cudaErrorInvalidDeviceFunction;
+  err = set_smem(kernel, C::kBytes, done);
   if (err != cudaSuccess) return err;
   int dev = 0, sms = 0;
   err = cudaGetDevice(&dev);
@@ -1063,8 +1070,7 @@ cudaError_t launch_chunk_kv(const SeqParams& p, cudaStream_t stream) {
   kernel<<<(unsigned)(units < sms ? units : sms), C::kThreads, C::kBytes, stream>>>(p, tmK, tmV);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1 || split_items == 0) return err;
-  join_kernel<D, kItemRows, kKeys><<<dim3((unsigned)split_items, kItemRows / 16), kJoinThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_join<D, kItemRows, kKeys>(p, dim3((unsigned)split_items, kItemRows / 16), stream);
 }
 
 }  // namespace

@@ -1,6 +1,8 @@
 // Joins the splits of the attention kernels' rows.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace solattn {
@@ -28,6 +30,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const KeyTiles kt = key_tiles<T>(p, sq.L, off + r_base / p.G, off + (r_base + rows - 1) / p.G);
   const int ns = max(1, min(p.splits, (kt.count() + p.unit - 1) / p.unit));
   if (ns == 1) return;
+  pdl_wait();
   const int64_t unit0 = (int64_t)blockIdx.x * p.splits;
   const float2* ml0 = reinterpret_cast<const float2*>(p.part + (int64_t)gridDim.x * p.splits * R * D);
   constexpr int kPer = D / 32;  // dims of a lane
@@ -59,6 +62,34 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
     for (int x = 0; x < kPer; x += 2)
       *reinterpret_cast<uint32_t*>(dst + x) = any ? pack_bf16(a[x] * inv, a[x + 1] * inv) : 0u;
   }
+}
+
+// Launches the join behind the kernel that was launched last on `stream`.
+template <int D, int R, int T>
+cudaError_t launch_join(const SeqParams& p, dim3 grid, cudaStream_t stream) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, join_kernel<D, R, T>, p);
+}
+
+// Once per device: the kernel's dynamic shared memory (`done` belongs to the kernel).
+template <typename K>
+cudaError_t set_smem(K* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (err == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return err;
 }
 
 }  // namespace solattn

@@ -67,6 +67,11 @@ __device__ __forceinline__ void note(int32_t* status, int code) {
   if (status) *reinterpret_cast<volatile int32_t*>(status) = code;
 }
 
+// Programmatic dependent launch: the join starts while its producer's last CTAs run, and waits for the
+// whole of it before it reads a result.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
 struct Seq {
   int b;      // sequence, or -1: the slot holds no rows
   int tile;   // the slot's row tile within the sequence
@@ -96,7 +101,7 @@ __device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) 
     return s;
   }
   int lo = 0, hi = p.B;  // the answer lies in [lo, hi)
-  int start = 0, next = 0;
+  int start = 0, next = 0, L = 0;
   while (true) {
     // Lane l probes b = lo + l * step.  The first probe (b = lo) always satisfies the condition.
     const int step = (hi - lo + 31) / 32;
@@ -104,6 +109,7 @@ __device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) 
     const bool in = b < hi;
     const int st = in ? __ldg(p.starts + b) : 0;
     const int en = (in && step == 1) ? __ldg(p.starts + b + 1) : 0;
+    const int len = (in && step == 1) ? __ldg(p.lengths + b) : 0;
     const bool le = in && (lane == 0 || slot_first(st, p.G, R, b) <= slot);
     const uint32_t bal = __ballot_sync(0xffffffffu, le);
     const int last = 31 - __clz(bal);
@@ -111,6 +117,7 @@ __device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) 
       s.b = lo + last;
       start = __shfl_sync(0xffffffffu, st, last);
       next = __shfl_sync(0xffffffffu, en, last);
+      L = __shfl_sync(0xffffffffu, len, last);
       break;
     }
     lo += last * step;
@@ -126,7 +133,6 @@ __device__ __forceinline__ Seq find_seq(const SeqParams& p, int slot, int lane) 
     s.n = s.L = s.tile = 0;
     return s;
   }
-  int L = __ldg(p.lengths + s.b);
   const int cap = p.width << p.page_shift;
   if (L < 0 || L > cap) {
     note(p.status, kStatusBadIndex);

@@ -20,6 +20,9 @@ namespace {
 
 constexpr int64_t kMaxKeys = int64_t(1) << 24;  // keys of a sequence, as in the routed entry points
 constexpr int64_t kSms = 148;
+#ifndef MINU
+#define MINU 256
+#endif
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
@@ -65,7 +68,7 @@ Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
   const int64_t chunk = D == 64 ? 32 : 16;  // keys of a chunk (rows.cu)
   const int64_t chunks = cdiv(keys, chunk) + 2;
   int64_t unit = cdiv(chunks * s.slots * Hkv, kSms * 2 * 4);
-  if (unit < 256 / chunk) unit = 256 / chunk;
+  if (unit < MINU / chunk) unit = MINU / chunk;
   if (unit > 2048 / chunk) unit = 2048 / chunk;
   if (unit < cdiv(chunks, 64)) unit = cdiv(chunks, 64);
   s.unit = unit;

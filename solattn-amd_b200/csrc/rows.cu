@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
   const int split = (int)(blockIdx.x % p.splits);
   const int h = (int)((blockIdx.x / p.splits) % p.Hkv);
   const int slot = (int)(blockIdx.x / ((unsigned)p.splits * p.Hkv));
+  pdl_trigger();
   if (split == 0 && h == 0 && p.zero_tail) zero_tail<D>(p, slot, p.slots, tid, kRowThreads);
   const Seq sq = find_seq<R>(p, slot, lane);
   if (sq.b < 0 || !p.takes(sq.n)) return;
@@ -599,14 +600,14 @@ template <int D, int KV, int R>
 cudaError_t launch_rows_kv(const SeqParams& p, cudaStream_t stream) {
   using C = RowsCfg<D, KV, R>;
   static_assert(C::kCtas * (C::kSmem + 1024) <= 227 * 1024, "CTAs that share an SM");
-  cudaError_t err = cudaFuncSetAttribute(rows_kernel<D, KV, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t err = set_smem(rows_kernel<D, KV, R>, C::kSmem, done);
   if (err != cudaSuccess) return err;
   const int64_t tiles = (int64_t)p.slots * p.Hkv;
   rows_kernel<D, KV, R><<<(unsigned)(tiles * p.splits), kRowThreads, C::kSmem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1) return err;
-  join_kernel<D, R, C::kChunk><<<(unsigned)tiles, kJoinThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_join<D, R, C::kChunk>(p, dim3((unsigned)tiles), stream);
 }
 
 template <int D, int R>

@@ -16,8 +16,8 @@ import torch
 
 from . import _lib
 from .attention import _is_b200, _nonnegative_integer
-from .status import monitor
-from .window import aligned, check_inputs, check_rule, check_scale, workspace
+from .status import error_word
+from .window import aligned, check_inputs, check_rule, check_scale, current_stream, on_device, workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
 
@@ -55,6 +55,7 @@ class PagedKVCache:
         if any(x.data_ptr() % 16 for x in xs):
             raise ValueError("Cache tensors must start on 16-byte boundaries")
         # What every launch passes on: page and scale addresses, pages, page size.
+        # (Kept here: the tensors may change their contents, not their places.)
         object.__setattr__(self, "_args", (
             self.k.data_ptr(), self.v.data_ptr(),
             None if self.k_scale is None else self.k_scale.data_ptr(),
@@ -122,6 +123,8 @@ class PagedPlan:
         if t.ndim != 2 or 0 in t.shape or n.shape != t.shape[:1] or s.shape != (t.shape[0] + 1,):
             raise ValueError("A plan holds page_table [B, width], key_lengths [B] and query_starts [B + 1]")
         _nonnegative_integer("most_new", self.most_new)
+        # What every launch passes on: the page table's address and width, the lengths' and the starts'.
+        object.__setattr__(self, "_args", (t.data_ptr(), t.shape[1], n.data_ptr(), s.data_ptr()))
 
     @classmethod
     def create(cls, page_table, key_lengths, query_starts, *, page_size=64, pages=None):
@@ -148,23 +151,16 @@ class PagedPlan:
                          self.most_new)
 
 
-def _check(cache, plan, *xs):
+def _check(cache, plan, x=None):
     """Checks shared by the operators; returns the device."""
     if not isinstance(cache, PagedKVCache) or not isinstance(plan, PagedPlan):
         raise ValueError("A PagedKVCache and a PagedPlan are required")
     device = cache.k.device
-    if device.type != "cuda" or any(x.device != device for x in xs) or not _is_b200(device):
+    if device.type != "cuda" or (x is not None and x.device != device) or not _is_b200(device):
         raise ValueError("The sm_100a backend requires the cache and Q/K/V on the same NVIDIA B200 CUDA GPU")
     if plan.page_table.device != device:
         raise ValueError("Transfer the plan to the cache's device first")
     return device
-
-
-def _on(device, fn, *args):
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return fn(*args)
-    return fn(*args)
 
 
 def cache_write(cache, plan, k, v):
@@ -177,22 +173,25 @@ def cache_write(cache, plan, k, v):
     if k.ndim != 3 or k.shape != v.shape or 0 in k.shape:
         raise ValueError("K/V must have matching nonempty [tokens, heads, D] shapes")
     check_inputs(k, v)
-    device = _check(cache, plan, k, v)
-    if k.shape[1:] != (cache.heads, cache.head_dim):
+    device = _check(cache, plan, k)
+    if v.device != device:
+        raise ValueError("The sm_100a backend requires the cache and Q/K/V on the same NVIDIA B200 CUDA GPU")
+    pages = cache.k.shape
+    if k.shape[1] != pages[1] or k.shape[2] != pages[3]:
         raise ValueError("K/V heads and dimension must match the cache")
-    _on(device, _write, cache, plan, k, v)
+    on_device(device, _write, cache, plan, k, v)
 
 
 def _write(cache, plan, k, v):
     k, v = aligned(k), aligned(v)
     N, H, D = k.shape
-    B, width = plan.page_table.shape
-    word = monitor(k.device).word()
+    index = k.device.index
+    sk, sv = k.stride(), v.stride()
     rc = _lib.load().solattn_cache_write(
-        k.data_ptr(), v.data_ptr(), N, H, D, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        *cache._args, plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(),
-        plan.query_starts.data_ptr(), B, word, torch.cuda.current_stream(k.device).cuda_stream)
-    _lib.check(rc, "solattn_cache_write")
+        k.data_ptr(), v.data_ptr(), N, H, D, sk[0], sk[1], sv[0], sv[1], *cache._args, *plan._args,
+        plan.page_table.shape[0], error_word(index), current_stream(index))
+    if rc:
+        _lib.check(rc, "solattn_cache_write")
 
 
 def cache_read(cache, plan, tokens):
@@ -203,20 +202,20 @@ def cache_read(cache, plan, tokens):
     if type(tokens) is not int or not 0 < tokens <= 1 << 24:
         raise ValueError("tokens must be a positive integer")
     device = _check(cache, plan)
-    return _on(device, _read, cache, plan, tokens)
+    return on_device(device, _read, cache, plan, tokens)
 
 
 def _read(cache, plan, tokens):
-    B, width = plan.page_table.shape
+    B = plan.page_table.shape[0]
+    _, H, _, D = cache.k.shape
     device = cache.k.device
-    word = monitor(device).word()
-    k, v = (torch.empty((B, tokens, cache.heads, cache.head_dim), dtype=torch.bfloat16, device=device)
-            for _ in range(2))
-    rc = _lib.load().solattn_cache_read(
-        *cache._args, plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(), B, cache.heads,
-        cache.head_dim, tokens, k.data_ptr(), v.data_ptr(), word,
-        torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, "solattn_cache_read")
+    word = error_word(device.index)
+    k = torch.empty((B, tokens, H, D), dtype=torch.bfloat16, device=device)
+    v = torch.empty((B, tokens, H, D), dtype=torch.bfloat16, device=device)
+    rc = _lib.load().solattn_cache_read(*cache._args, *plan._args[:3], B, H, D, tokens, k.data_ptr(),
+                                        v.data_ptr(), word, current_stream(device.index))
+    if rc:
+        _lib.check(rc, "solattn_cache_read")
     return k, v
 
 
@@ -235,30 +234,33 @@ def paged_attention(q, cache, plan, *, window=None, lookahead=0, sink_tokens=0, 
         raise ValueError("Q must be a nonempty packed [tokens, heads, D] tensor")
     check_inputs(q)
     device = _check(cache, plan, q)
-    if q.shape[2] != cache.head_dim or q.shape[1] % cache.heads != 0:
+    N, Hq, D = q.shape
+    _, Hkv, page, cache_dim = cache.k.shape
+    if D != cache_dim or Hq % Hkv:
         raise ValueError("Q's dimension must match the cache and its heads be a multiple of the cache's")
-    scale = check_scale(scale, q.shape[2])
+    scale = check_scale(scale, D)
     rule = check_rule(window, lookahead, sink_tokens)
     if out is not None and (out.dtype != torch.bfloat16 or out.device != device or out.shape != q.shape
                             or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
-    return _on(device, _attend, q, cache, plan, rule, scale, out)
+    return on_device(device, _attend, q, cache, plan, rule, scale, out, (N, Hq, Hkv, D, page))
 
 
-def _attend(q, cache, plan, rule, scale, out):
+def _attend(q, cache, plan, rule, scale, out, shape):
     q = aligned(q)
-    N, Hq, D = q.shape
+    N, Hq, Hkv, D, page = shape
+    device = q.device
     B, width = plan.page_table.shape
-    fresh = out is None
-    word = monitor(q.device).word()
+    word = error_word(device.index)  # an earlier call's device-side error surfaces here
     keep, ws, size = workspace("solattn_paged_workspace_bytes",
-                               (N, B, Hq, cache.heads, D, cache.page_size, width, plan.most_new, *rule), q.device)
+                               (N, B, Hq, Hkv, D, page, width, plan.most_new) + rule, device)
+    fresh = out is None
     if fresh:
-        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=device)
+    sq = q.stride()
     rc = _lib.load().solattn_paged_attention(
-        q.data_ptr(), N, Hq, cache.heads, D, q.stride(0), q.stride(1), *cache._args,
-        plan.page_table.data_ptr(), width, plan.key_lengths.data_ptr(), plan.query_starts.data_ptr(), B,
-        plan.most_new, *rule, scale, int(fresh), ws, size, out.data_ptr(), word,
-        torch.cuda.current_stream(q.device).cuda_stream)
-    _lib.check(rc, "solattn_paged_attention")
+        q.data_ptr(), N, Hq, Hkv, D, sq[0], sq[1], *cache._args, *plan._args, B, plan.most_new, *rule, scale,
+        fresh, ws, size, out.data_ptr(), word, current_stream(device.index))
+    if rc:
+        _lib.check(rc, "solattn_paged_attention")
     return out

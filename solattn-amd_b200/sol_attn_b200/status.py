@@ -138,6 +138,12 @@ def monitor(device: torch.device) -> StatusMonitor:
         return _MONITORS[index]
 
 
+def error_word(index: int) -> int:
+    """``StatusMonitor.word()`` of device ``index`` (the short way of every call)."""
+    mon = _MONITORS.get(index)
+    return (mon if mon is not None else monitor(torch.device("cuda", index))).word()
+
+
 def check_device_errors(device=None) -> None:
     """Wait for every pending status copy (of ``device``, or of every device used) and raise
     :class:`DeviceError` if a call reported a device-side error."""

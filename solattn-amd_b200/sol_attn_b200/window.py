@@ -13,7 +13,10 @@ import torch
 
 from . import _lib
 from .attention import _aligned, _is_b200
-from .status import monitor
+from .status import error_word
+
+# The current stream's handle without the stream object around it (a third of a small call's cost).
+current_stream = torch._C._cuda_getCurrentRawStream
 
 # Window and lookahead without a bound, in the C ABI.
 _NO_WINDOW, _NO_LOOKAHEAD = 0, -1
@@ -37,7 +40,9 @@ def check_rule(window, lookahead, sink_tokens):
 
 
 def check_scale(scale, dim):
-    scale = dim ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        return dim ** -0.5
+    scale = float(scale)
     if not math.isfinite(scale) or scale <= 0:
         raise ValueError("scale must be finite and positive")
     return scale
@@ -45,14 +50,14 @@ def check_scale(scale, dim):
 
 def workspace(fn, key, device):
     """(tensor or None, address, bytes) of a call's scratch; its size is cached per shape."""
-    size = _WORKSPACE.get((fn, key))
+    size = _WORKSPACE.get(key)
     if size is None:
         size = getattr(_lib.load(), fn)(*key)
         if size < 0:
             raise _lib.SolAttnError("unsupported shape for libsolattn")
         if len(_WORKSPACE) >= 4096:
             _WORKSPACE.clear()
-        _WORKSPACE[(fn, key)] = size
+        _WORKSPACE[key] = size
     if size == 0:
         return None, None, 0
     x = torch.empty(size, dtype=torch.uint8, device=device)
@@ -68,14 +73,23 @@ def aligned(x):
 def check_inputs(*xs):
     """Checks shared by the inference-only BF16 operators beyond their shapes."""
     for x in xs:
-        if x.dtype != torch.bfloat16:
+        if x.dtype is not torch.bfloat16:
             raise ValueError("Only BF16 Q/K/V are implemented")
         if x.requires_grad:
             raise ValueError("Inference only: Q/K/V must not require gradients")
-        if x.stride(-1) != 1 or min(x.stride()) <= 0:
+        strides = x.stride()
+        if strides[-1] != 1 or min(strides) <= 0:
             raise ValueError("Q/K/V need positive strides and contiguous head dimension")
     if xs[0].shape[-1] not in (64, 128):
         raise ValueError("Only head dimensions 64 and 128 are implemented")
+
+
+def on_device(device, fn, *args):
+    """``fn(*args)`` with ``device`` current."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return fn(*args)
+    return fn(*args)
 
 
 def window_attention(q, k, v, *, window=None, lookahead=0, sink_tokens=0, scale=None):
@@ -88,35 +102,33 @@ def window_attention(q, k, v, *, window=None, lookahead=0, sink_tokens=0, scale=
     ``window`` counts the query's own position.  A query that sees no key gives zeros, and keys that a
     query does not see have no influence on it whatever they hold.  FP32 softmax and sums.
     """
-    if any(t.ndim != 4 for t in (q, k, v)):
+    if q.ndim != 4 or k.ndim != 4 or v.ndim != 4:
         raise ValueError("Q/K/V must have BTHD rank-4 layout")
-    if (k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]
-            or any(n <= 0 for n in q.shape + k.shape) or q.shape[2] % k.shape[2] != 0):
+    B, Tq, Hq, D = q.shape
+    Bk, Tk, Hkv, Dk = k.shape
+    if k.shape != v.shape or B != Bk or D != Dk or 0 in (B, Tq, Hq, D, Tk, Hkv) or Hq % Hkv:
         raise ValueError("Q/K/V batch and dimension shapes must agree and be nonempty, and Q heads "
                          "be a multiple of K/V heads")
     check_inputs(q, k, v)
-    scale = check_scale(scale, q.shape[3])
+    scale = check_scale(scale, D)
     rule = check_rule(window, lookahead, sink_tokens)
     device = q.device
     if (device.type != "cuda" or k.device != device or v.device != device
             or not _is_b200(device)):
         raise ValueError("The sm_100a backend requires Q/K/V on the same NVIDIA B200 CUDA GPU")
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _launch(q, k, v, rule, scale)
-    return _launch(q, k, v, rule, scale)
+    return on_device(device, _launch, q, k, v, rule, scale, (B, Tq, Tk, Hq, Hkv, D))
 
 
-def _launch(q, k, v, rule, scale):
-    q, k, v = (aligned(x) for x in (q, k, v))
-    B, Tq, Hq, D = q.shape
-    Tk, Hkv = k.shape[1], k.shape[2]
-    word = monitor(q.device).word()  # an earlier call's device-side error surfaces here
-    keep, ws, size = workspace("solattn_window_workspace_bytes", (B, Tq, Tk, Hq, Hkv, D, *rule), q.device)
-    out = torch.empty((B, Tq, Hq, D), dtype=torch.bfloat16, device=q.device)
+def _launch(q, k, v, rule, scale, shape):
+    q, k, v = aligned(q), aligned(k), aligned(v)
+    device = q.device
+    word = error_word(device.index)  # an earlier call's device-side error surfaces here
+    keep, ws, size = workspace("solattn_window_workspace_bytes", shape + rule, device)
+    out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
+    sq, sk, sv = q.stride(), k.stride(), v.stride()
     rc = _lib.load().solattn_window_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), B, Tq, Tk, Hq, Hkv, D, *q.stride()[:3],
-        *k.stride()[:3], *v.stride()[:3], *rule, scale, ws, size, out.data_ptr(), word,
-        torch.cuda.current_stream(q.device).cuda_stream)
-    _lib.check(rc, "solattn_window_attention")
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, sq[0], sq[1], sq[2], sk[0], sk[1], sk[2],
+        sv[0], sv[1], sv[2], *rule, scale, ws, size, out.data_ptr(), word, current_stream(device.index))
+    if rc:
+        _lib.check(rc, "solattn_window_attention")
     return out
