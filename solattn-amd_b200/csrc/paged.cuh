@@ -41,7 +41,8 @@ struct SeqParams {
   int B, N, Hq, Hkv, G, Tq, Tk;  // N: rows of q over all sequences (B * Tq when contiguous)
   int window, ahead, sinks;
   int slots, splits, unit;  // row tiles over all sequences; splits of a tile; key tiles per split
-  int first;                // items (a slot and a K/V head) from this number on are split
+  int cluster;              // few-rows kernel: the splits of a tile are a cluster
+  int first;                // chunk kernel: items (a slot and a K/V head) from this number on are split
   int zero_tail;            // write zeros to the rows behind the last sequence
   int min_new, max_new;     // new tokens of the sequences that this launch takes
   float scale_log2;         // softmax scale * log2(e)

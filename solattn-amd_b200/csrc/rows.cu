@@ -8,8 +8,8 @@
 // its own cp.async ring (no CTA barrier in the loop) and keeps its own m, l and O in registers; the
 // warps merge at the end.  The products run on mma.sync m16n8k16: with so few rows the tensor work is a
 // few per cent of the time that the bytes take, and the fragments need no shared-memory round trip
-// of S and P.  Long sequences are split over several CTAs (`unit` chunks each), whose partial
-// results a second kernel joins in a fixed order.
+// of S and P.  Long sequences are split over several CTAs (`unit` chunks each).  Up to 8 of them
+// form a cluster and join their results through its shared memory; with more, a second kernel joins them.
 //
 // Keys that a row does not see have no influence whatever they hold: S is replaced by -inf, and a
 // chunk with a non-finite V (where P = 0 times V would be NaN) goes through exact_pv, which adds
@@ -42,7 +42,8 @@ struct RowsCfg {
   static constexpr int kCtas = KV != kPagedE4m3 ? 2 : D == 64 ? 4 : 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kMerge = kWarps * R * (D + 2) * 4;  // m, l, O of every warp
-  static constexpr int kSmem = kWarps * kRing > kMerge ? kWarps * kRing : kMerge;
+  static constexpr int kSmem = kWarps * kRing;
+  static_assert(kSmem >= kMerge + R * (D + 2) * 4, "the results of the warps, and of the CTA, over the rings");
   static constexpr int kHalves = R / 8;  // row groups g and g + 8 of the MMA
 };
 
@@ -126,6 +127,30 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A barrier of the cluster, after which its CTAs see each other's shared memory as it was written before.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// The address of `addr` (own shared memory) in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
 // O += P V of one chunk whose V is not finite (or, E4M3, whose scales lie too far apart), key by key and
 // only where the row sees the key.  `scales` is the chunk's V exponents, O holds 2^(127 + 13 - ref) of
 // its value (E4M3).
@@ -199,7 +224,13 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
   const KeyTiles kt = key_tiles<C::kChunk>(p, sq.L, pos0, pos1);
   const int total = kt.count();
   const int ns = max(1, min(p.splits, (total + p.unit - 1) / p.unit));
-  if (split >= ns) return;
+  if (split >= ns) {
+    if (p.cluster) {  // (its cluster waits for it twice)
+      cluster_sync();
+      cluster_sync();
+    }
+    return;
+  }
   const int c0 = (int)((int64_t)total * split / ns), c1 = (int)((int64_t)total * (split + 1) / ns);
   const int mine = c1 - c0 > warp ? (c1 - c0 - warp + kWarps - 1) / kWarps : 0;  // this warp's chunks
   // Keys that some row sees: [low, high] and those below the sinks.
@@ -556,6 +587,18 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
   }
   __syncthreads();
   const int64_t unit = ((int64_t)slot * p.Hkv + h) * p.splits + split;
+  float* sPart = reinterpret_cast<float*>(smem + C::kMerge);  // cluster: this CTA's O [row][D], then m, l
+  auto store = [&](int r, int d, const float4& a, float sum) {
+    const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
+    // A row that sees no key gives zeros.
+    const int top = key_high(p, sq.L, pos);
+    const bool any = top >= 0 && (top >= key_low(p, pos) || p.sinks > 0);
+    const float inv = any ? 1.f / sum : 0.f;
+    uint2 w;
+    w.x = any ? pack_bf16(a.x * inv, a.y * inv) : 0u;
+    w.y = any ? pack_bf16(a.z * inv, a.w * inv) : 0u;
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + d) = w;
+  };
   for (int i = tid; i < rows * (D / 4); i += kRowThreads) {
     const int r = i / (D / 4), d = 4 * (i % (D / 4));
     float mx = -INFINITY, sum = 0.f;
@@ -573,7 +616,13 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
       a.z += x.z * f;
       a.w += x.w * f;
     }
-    if (ns > 1) {
+    if (ns > 1 && p.cluster) {
+      *reinterpret_cast<float4*>(sPart + r * D + d) = a;
+      if (d == 0) {
+        sPart[R * D + 2 * r] = mx;
+        sPart[R * D + 2 * r + 1] = sum;
+      }
+    } else if (ns > 1) {
       *reinterpret_cast<float4*>(p.part + (unit * R + r) * D + d) = a;
       if (d == 0) {
         float* ml = p.part + (int64_t)p.slots * p.Hkv * p.splits * R * D + (unit * R + r) * 2;
@@ -581,17 +630,35 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
         ml[1] = sum;
       }
     } else {
-      const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
-      // A row that sees no key gives zeros.
-      const int top = key_high(p, sq.L, pos);
-      const bool any = top >= 0 && (top >= key_low(p, pos) || p.sinks > 0);
-      const float inv = any ? 1.f / sum : 0.f;
-      uint2 w;
-      w.x = any ? pack_bf16(a.x * inv, a.y * inv) : 0u;
-      w.y = any ? pack_bf16(a.z * inv, a.w * inv) : 0u;
-      *reinterpret_cast<uint2*>(p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + d) = w;
+      store(r, d, a, sum);
     }
   }
+  if (!p.cluster) return;
+  // ---- the cluster's CTAs hold the splits of one tile: each joins its share of the rows' pieces from the
+  // others' shared memory, in the order of the splits (the result does not depend on who does it).
+  cluster_sync();
+  if (ns > 1) {
+    const uint32_t part = smem_u32(sPart);
+    for (int i = tid + kRowThreads * split; i < rows * (D / 4); i += kRowThreads * ns) {
+      const int r = i / (D / 4), d = 4 * (i % (D / 4));
+      float mx = -INFINITY, sum = 0.f;
+      for (int x = 0; x < ns; ++x) mx = fmaxf(mx, ld_cluster(cluster_addr(part + (uint32_t)(R * D + 2 * r) * 4u, x)));
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = 0; x < ns; ++x) {
+        const uint32_t ml = cluster_addr(part + (uint32_t)(R * D + 2 * r) * 4u, x);
+        const float f = fast_exp2(ld_cluster(ml) - base);
+        sum += ld_cluster(ml + 4u) * f;
+        const float4 o4 = ld_cluster4(cluster_addr(part + (uint32_t)(r * D + d) * 4u, x));
+        a.x += o4.x * f;
+        a.y += o4.y * f;
+        a.z += o4.z * f;
+        a.w += o4.w * f;
+      }
+      store(r, d, a, sum);
+    }
+  }
+  cluster_sync();  // nobody leaves while its shared memory is read
 }
 
 namespace {
@@ -604,6 +671,20 @@ cudaError_t launch_rows_kv(const SeqParams& p, cudaStream_t stream) {
   cudaError_t err = set_smem(rows_kernel<D, KV, R>, C::kSmem, done);
   if (err != cudaSuccess) return err;
   const int64_t tiles = (int64_t)p.slots * p.Hkv;
+  if (p.cluster) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)p.splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * p.splits));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, rows_kernel<D, KV, R>, p);
+  }
   rows_kernel<D, KV, R><<<(unsigned)(tiles * p.splits), kRowThreads, C::kSmem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1) return err;

@@ -165,11 +165,11 @@ def test_cache_entry_points_reject():
 
 
 def test_workspace_sizes():
-    """Short calls need none; long ones hold 8 or 16 rows of D + 2 floats per split."""
+    """Calls of few splits need none; long ones hold 8 or 16 rows of D + 2 floats per split."""
     L = _lib.load()
     assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 2, 64, 0, 0, 0) == 0
     assert L.solattn_window_workspace_bytes(1, 1, 100, 4, 3, 64, 0, 0, 0) == -1
-    size = L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 16, 1, 0, 0, 0)
+    size = L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 300, 1, 0, 0, 0)
     assert size > 0 and size % (8 * 130 * 4) == 0
     # A window bounds what is split, however wide the table is.
     assert L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 1 << 18, 1, 64, 0, 4) == 0
