@@ -15,6 +15,7 @@ namespace solattn {
 namespace {
 
 constexpr int kCopyThreads = 256;
+constexpr int kRun = 4;  // rows of a group of lanes (read of 32768 x 24 E4M3 rows: 1, 2, 4: 147, 110, 95 us)
 
 // 448 * 2^e >= top for the least e, as the biased exponent e + 127 clamped to [0, 254]: with top =
 // f * 2^x, 1 <= f < 2, that is x - 8 where f <= 1.75, else x - 7.
@@ -48,101 +49,182 @@ __device__ __forceinline__ int seq_of_token(const CacheParams& p, int tok) {
 
 }  // namespace
 
-// Row (token, head) of K or V per group of D / 8 lanes.
+// kRun consecutive rows (token, head) of K or V per group of D / 8 lanes, all loads before the first store.
 template <int D, bool kE4m3>
 __global__ void __launch_bounds__(kCopyThreads) cache_write_kernel(const CacheParams p) {
   constexpr int kLanes = D / 8;
-  const int sub = threadIdx.x % kLanes;
-  const int64_t rows = (int64_t)p.N * p.Hkv;
-  const int64_t row = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) / kLanes;
-  const int z = blockIdx.y;
-  const bool in = row < rows;
-  const int tok = in ? (int)(row / p.Hkv) : 0, h = in ? (int)(row % p.Hkv) : 0;
-  const uint4 raw = in ? __ldg(reinterpret_cast<const uint4*>(p.x[z] + (int64_t)tok * p.sT[z] + (int64_t)h * p.sH[z]) + sub)
-                       : make_uint4(0, 0, 0, 0);
-  const int b = seq_of_token(p, tok);
-  const int start = __ldg(p.starts + b), next = __ldg(p.starts + b + 1);
-  bool ok = in && tok >= start && tok < next;  // rows behind the last sequence are left out
-  int64_t dst = 0;
-  if (ok) {
-    const int pos = __ldg(p.lengths + b) - next + tok;
-    int page = -1;
-    if (pos >= 0 && pos < (p.width << p.page_shift))
-      page = __ldg(p.table + (int64_t)b * p.width + (pos >> p.page_shift));
-    if (start < 0 || next > p.N || page < 0 || page >= p.npages) {
-      note(p.status, kStatusBadIndex);
-      ok = false;
-    } else {
-      dst = (((int64_t)page * p.Hkv + h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+  const int sub = threadIdx.x % kLanes, z = blockIdx.y;
+  const uint32_t rows = (uint32_t)p.N * (uint32_t)p.Hkv;  // (below 2^31: checked by the host)
+  const uint32_t row0 = (blockIdx.x * (uint32_t)(kCopyThreads / kLanes) + threadIdx.x / kLanes) * kRun;
+  const uint32_t first = min(row0, rows - 1);
+  const int tok0 = (int)(first / (uint32_t)p.Hkv), h0 = (int)(first % (uint32_t)p.Hkv);
+  uint4 raw[kRun];
+  int tok = tok0, h = h0;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    raw[j] = make_uint4(0, 0, 0, 0);
+    if (row0 + j < rows)
+      raw[j] = __ldg(reinterpret_cast<const uint4*>(p.x[z] + (int64_t)tok * p.sT[z] + (int64_t)h * p.sH[z]) + sub);
+    if (++h == p.Hkv) {
+      h = 0;
+      ++tok;
+    }
+  }
+  // Their places in the cache (rows of it), or -1.  The heads of a token are a page's rows apart, so
+  // that the token is looked up once.
+  int64_t dst[kRun];
+  int start = 0, next = 0, last = 0, b = -1;  // the token's sequence: its packed tokens, key_lengths - next
+  int64_t at = -1;
+  tok = tok0;
+  h = h0;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    if (row0 + j < rows && (j == 0 || h == 0)) {
+      if (b < 0 || tok >= next || tok < start) {
+        b = seq_of_token(p, tok);
+        start = __ldg(p.starts + b);
+        next = __ldg(p.starts + b + 1);
+        last = __ldg(p.lengths + b) - next;
+      }
+      at = -1;
+      if (tok >= start && tok < next) {  // (rows behind the last sequence are left out)
+        const int pos = last + tok;
+        int page = -1;
+        if (pos >= 0 && pos < (p.width << p.page_shift))
+          page = __ldg(p.table + (int64_t)b * p.width + (pos >> p.page_shift));
+        if (start < 0 || next > p.N || page < 0 || page >= p.npages) note(p.status, kStatusBadIndex);
+        else at = (((int64_t)page * p.Hkv + h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+      }
+    }
+    dst[j] = row0 + j < rows ? at : -1;
+    if (at >= 0) at += int64_t(1) << p.page_shift;
+    if (++h == p.Hkv) {
+      h = 0;
+      ++tok;
     }
   }
   if constexpr (!kE4m3) {
-    if (ok) reinterpret_cast<uint4*>(p.pages[z] + dst * D * 2)[sub] = raw;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      if (dst[j] >= 0) reinterpret_cast<uint4*>(p.pages[z] + dst[j] * D * 2)[sub] = raw[j];
   } else {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float top = 0.f;
+    // The largest magnitude of a row, as BF16 bits (which order like the values), pairs at a time.
+    uint32_t top[kRun];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float lo = fabsf(__uint_as_float(w[i] << 16)), hi = fabsf(__uint_as_float(w[i] & 0xffff0000u));
-      if (lo < INFINITY) top = fmaxf(top, lo);
-      if (hi < INFINITY) top = fmaxf(top, hi);
-    }
+    for (int j = 0; j < kRun; ++j) {
+      top[j] = __vimax3_u16x2(raw[j].x & 0x7fff7fffu, raw[j].y & 0x7fff7fffu, raw[j].z & 0x7fff7fffu);
+      top[j] = __vimax3_u16x2(top[j], top[j], raw[j].w & 0x7fff7fffu);
+      if ((top[j] & 0xffffu) >= 0x7f80u || (top[j] >> 16) >= 0x7f80u) {  // (rare) not finite: left out
+        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+        top[j] = 0u;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const int e = scale_exponent(top);
-    if (ok) {
-      const uint2 c = to_e4m3(raw, __uint_as_float((uint32_t)(254 - e) << 23));
-      reinterpret_cast<uint2*>(p.pages[z] + dst * D)[sub] = c;
-      if (sub == 0) p.scale[z][dst] = (uint8_t)e;
-    }
-  }
-}
-
-// Row (sequence, token, head) of K or V per group of D / 8 lanes; zeros behind a sequence's end.
-template <int D, bool kE4m3>
-__global__ void __launch_bounds__(kCopyThreads) cache_read_kernel(const CacheParams p) {
-  constexpr int kLanes = D / 8;
-  const int sub = threadIdx.x % kLanes;
-  const int64_t row = ((int64_t)blockIdx.x * kCopyThreads + threadIdx.x) / kLanes;
-  const int z = blockIdx.y;
-  if (row >= (int64_t)p.B * p.tokens * p.Hkv) return;
-  const int h = (int)(row % p.Hkv);
-  const int64_t bt = row / p.Hkv;
-  const int b = (int)(bt / p.tokens), pos = (int)(bt % p.tokens);
-  int L = __ldg(p.lengths + b);
-  const int cap = p.width << p.page_shift;
-  if (L < 0 || L > cap) {
-    note(p.status, kStatusBadIndex);
-    L = L < 0 ? 0 : cap;
-  }
-  uint4 out = make_uint4(0, 0, 0, 0);
-  if (pos < L) {
-    const int page = __ldg(p.table + (int64_t)b * p.width + (pos >> p.page_shift));
-    if (page < 0 || page >= p.npages) {
-      note(p.status, kStatusBadIndex);
-    } else {
-      const int64_t src = (((int64_t)page * p.Hkv + h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
-      if constexpr (!kE4m3) {
-        out = __ldg(reinterpret_cast<const uint4*>(p.pages[z] + src * D * 2) + sub);
-      } else {
-        const uint2 c = __ldg(reinterpret_cast<const uint2*>(p.pages[z] + src * D) + sub);
-        const float f = e8m0_value(p.scale[z][src]);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = ((i & 2) ? c.y : c.x) >> (16 * (i & 1));
-          w[i] = pack_bf16(e4m3_value(two & 0xffu) * f, e4m3_value((two >> 8) & 0xffu) * f);
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t m = (w[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+          if (m < 0x7f80u) top[j] = max(top[j], m);
         }
-        out = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) top[j] = __vimax3_u16x2(top[j], top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const int e = scale_exponent(__uint_as_float(max(top[j] & 0xffffu, top[j] >> 16) << 16));
+      const uint2 c = to_e4m3(raw[j], __uint_as_float((uint32_t)(254 - e) << 23));
+      if (dst[j] >= 0) {
+        reinterpret_cast<uint2*>(p.pages[z] + dst[j] * D)[sub] = c;
+        if (sub == 0) p.scale[z][dst[j]] = (uint8_t)e;
       }
     }
   }
-  reinterpret_cast<uint4*>(p.y[z] + row * D)[sub] = out;
+}
+
+// kRun consecutive rows (sequence, token, head) of K or V per group of D / 8 lanes; zeros behind a
+// sequence's end.
+template <int D, bool kE4m3>
+__global__ void __launch_bounds__(kCopyThreads) cache_read_kernel(const CacheParams p) {
+  constexpr int kLanes = D / 8;
+  const int sub = threadIdx.x % kLanes, z = blockIdx.y;
+  const uint32_t rows = (uint32_t)p.B * (uint32_t)p.tokens * (uint32_t)p.Hkv;  // (below 2^31)
+  const uint32_t row0 = (blockIdx.x * (uint32_t)(kCopyThreads / kLanes) + threadIdx.x / kLanes) * kRun;
+  if (row0 >= rows) return;
+  int h = (int)(row0 % (uint32_t)p.Hkv);
+  const uint32_t bt = row0 / (uint32_t)p.Hkv;
+  int b = (int)(bt / (uint32_t)p.tokens), pos = (int)(bt % (uint32_t)p.tokens);
+  const int cap = p.width << p.page_shift;
+  int64_t src[kRun];  // cache row, or -1; a token is looked up once
+  int L = -1;
+  int64_t at = -1;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    if (row0 + j < rows && (j == 0 || h == 0)) {
+      if (L < 0) {
+        L = __ldg(p.lengths + b);
+        if (L < 0 || L > cap) {
+          note(p.status, kStatusBadIndex);
+          L = L < 0 ? 0 : cap;
+        }
+      }
+      at = -1;
+      if (pos < L) {
+        const int page = __ldg(p.table + (int64_t)b * p.width + (pos >> p.page_shift));
+        if (page < 0 || page >= p.npages) note(p.status, kStatusBadIndex);
+        else at = (((int64_t)page * p.Hkv + h) << p.page_shift) + (pos & ((1 << p.page_shift) - 1));
+      }
+    }
+    src[j] = row0 + j < rows ? at : -1;
+    if (at >= 0) at += int64_t(1) << p.page_shift;
+    if (++h == p.Hkv) {
+      h = 0;
+      if (++pos == p.tokens) {
+        pos = 0;
+        ++b;
+        L = -1;
+      }
+    }
+  }
+  uint4* out = reinterpret_cast<uint4*>(p.y[z] + (int64_t)row0 * D) + sub;
+  if constexpr (!kE4m3) {
+    uint4 raw[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      raw[j] = src[j] >= 0 ? __ldg(reinterpret_cast<const uint4*>(p.pages[z] + src[j] * D * 2) + sub) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      if (row0 + j < rows) out[j * kLanes] = raw[j];
+  } else {
+    uint2 c[kRun];
+    uint32_t e[kRun];
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      c[j] = src[j] >= 0 ? __ldg(reinterpret_cast<const uint2*>(p.pages[z] + src[j] * D) + sub) : make_uint2(0, 0);
+      e[j] = src[j] >= 0 ? __ldg(p.scale[z] + src[j]) : 127u;
+    }
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const float f = e8m0_value(e[j]);
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t two = (uint16_t)(((i & 2) ? c[j].y : c[j].x) >> (16 * (i & 1)));
+        const __half2_raw h2 = __nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3);  // exact; NaN stays NaN
+        const float2 v = __half22float2(__half2(h2));
+        w[i] = pack_bf16(v.x * f, v.y * f);
+      }
+      if (row0 + j < rows) out[j * kLanes] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// Blocks for `rows` rows.
+static unsigned copy_blocks(int64_t rows, int D) {
+  const int64_t per = (int64_t)(kCopyThreads / (D / 8)) * kRun;
+  return (unsigned)((rows + per - 1) / per);
 }
 
 cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream) {
-  const int64_t threads = (int64_t)p.N * p.Hkv * (D / 8);
-  const dim3 grid((unsigned)((threads + kCopyThreads - 1) / kCopyThreads), 2);
+  const dim3 grid(copy_blocks((int64_t)p.N * p.Hkv, D), 2);
   if (D == 128) {
     if (p.scale[0]) cache_write_kernel<128, true><<<grid, kCopyThreads, 0, stream>>>(p);
     else cache_write_kernel<128, false><<<grid, kCopyThreads, 0, stream>>>(p);
@@ -154,8 +236,7 @@ cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream)
 }
 
 cudaError_t launch_cache_read(const CacheParams& p, int D, cudaStream_t stream) {
-  const int64_t threads = (int64_t)p.B * p.tokens * p.Hkv * (D / 8);
-  const dim3 grid((unsigned)((threads + kCopyThreads - 1) / kCopyThreads), 2);
+  const dim3 grid(copy_blocks((int64_t)p.B * p.tokens * p.Hkv, D), 2);
   if (D == 128) {
     if (p.scale[0]) cache_read_kernel<128, true><<<grid, kCopyThreads, 0, stream>>>(p);
     else cache_read_kernel<128, false><<<grid, kCopyThreads, 0, stream>>>(p);

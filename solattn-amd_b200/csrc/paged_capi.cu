@@ -347,7 +347,7 @@ int solattn_cache_write(const void* k, const void* v, int64_t N, int64_t Hkv, in
   if (!k || !v || !query_starts || N <= 0 || !aligned16(k) || !aligned16(v) || !stride_ok(k_sT) ||
       !stride_ok(k_sH) || !stride_ok(v_sT) || !stride_ok(v_sH))
     return SOLATTN_ERR_ARG;
-  if (N > 0x7fffffff || cdiv(N * Hkv * (D / 8), 256) >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  if (N > 0x7fffffff || N * Hkv > 0x7fffffff) return SOLATTN_ERR_ARG;  // (2^31 rows are 256 GB and more)
   p.x[0] = static_cast<const __nv_bfloat16*>(k);
   p.x[1] = static_cast<const __nv_bfloat16*>(v);
   p.sT[0] = k_sT, p.sT[1] = v_sT;
@@ -366,7 +366,7 @@ int solattn_cache_read(const void* k_pages, const void* v_pages, const void* k_s
                               table_width, key_lengths, status);
   if (rc) return rc;
   if (!k || !v || !aligned16(k) || !aligned16(v) || tokens <= 0 || tokens > kMaxKeys) return SOLATTN_ERR_ARG;
-  if (cdiv(B * tokens * Hkv, 256) * (D / 8) >= (int64_t(1) << 31)) return SOLATTN_ERR_ARG;
+  if (B * tokens > 0x7fffffff || B * tokens * Hkv > 0x7fffffff) return SOLATTN_ERR_ARG;
   p.y[0] = static_cast<__nv_bfloat16*>(k);
   p.y[1] = static_cast<__nv_bfloat16*>(v);
   p.tokens = (int)tokens;
