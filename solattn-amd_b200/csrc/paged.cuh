@@ -209,14 +209,6 @@ __device__ __forceinline__ float e8m0_value(uint32_t e) {
   return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7fc00000u : e << 23);
 }
 
-// Two E4M3 codes in the high bytes of the 16-bit halves of x -> the same bits in BF16's fields: a
-// BF16 pair that is 2^-120 times the two values (the formats differ by 120 in exponent bias, and
-// E4M3's subnormals become BF16's).
-__device__ __forceinline__ uint32_t e4m3_fields(uint32_t x) {
-  return ((x >> 4) & 0x07f007f0u) | (x & 0x80008000u);
-}
-constexpr uint32_t kTwo120x2 = 0x7b807b80u;  // BF16 pair of 2^120
-
 __device__ __forceinline__ uint32_t bf16x2_mul(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -234,11 +226,6 @@ __device__ __forceinline__ float e4m3_value(uint32_t c) {
   if (mag == 0x7fu) return __uint_as_float(0x7fc00000u);
   const float v = __uint_as_float(mag << 20) * __uint_as_float(247u << 23);  // fields, then 2^120
   return (c & 0x80u) ? -v : v;
-}
-
-// Bytes equal to 0x7f or 0xff (E4M3's NaN) in any of the four: nonzero.
-__device__ __forceinline__ uint32_t e4m3_nan_bytes(uint32_t w) {
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
 }  // namespace solattn

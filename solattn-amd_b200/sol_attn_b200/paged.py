@@ -54,13 +54,13 @@ class PagedKVCache:
             raise ValueError("Cache tensors must be contiguous and on one device")
         if any(x.data_ptr() % 16 for x in xs):
             raise ValueError("Cache tensors must start on 16-byte boundaries")
-        # What every launch passes on: page and scale addresses, pages, page size.
-        # (Kept here: the tensors may change their contents, not their places.)
-        object.__setattr__(self, "_args", (
-            self.k.data_ptr(), self.v.data_ptr(),
-            None if self.k_scale is None else self.k_scale.data_ptr(),
-            None if self.v_scale is None else self.v_scale.data_ptr(),
-            self.k.shape[0], self.k.shape[2]))
+
+    def _args(self):
+        """What every launch passes on: page and scale addresses, pages, page size."""
+        ks, vs = self.k_scale, self.v_scale
+        shape = self.k.shape
+        return (self.k.data_ptr(), self.v.data_ptr(), None if ks is None else ks.data_ptr(),
+                None if vs is None else vs.data_ptr(), shape[0], shape[2])
 
     @classmethod
     def create(cls, pages, heads, head_dim, *, page_size=64, dtype=torch.bfloat16, device="cuda"):
@@ -123,8 +123,11 @@ class PagedPlan:
         if t.ndim != 2 or 0 in t.shape or n.shape != t.shape[:1] or s.shape != (t.shape[0] + 1,):
             raise ValueError("A plan holds page_table [B, width], key_lengths [B] and query_starts [B + 1]")
         _nonnegative_integer("most_new", self.most_new)
-        # What every launch passes on: the page table's address and width, the lengths' and the starts'.
-        object.__setattr__(self, "_args", (t.data_ptr(), t.shape[1], n.data_ptr(), s.data_ptr()))
+
+    def _args(self):
+        """What every launch passes on: the page table's address and width, the lengths' and the starts'."""
+        t = self.page_table
+        return t.data_ptr(), t.shape[1], self.key_lengths.data_ptr(), self.query_starts.data_ptr()
 
     @classmethod
     def create(cls, page_table, key_lengths, query_starts, *, page_size=64, pages=None):
@@ -163,6 +166,13 @@ def _check(cache, plan, x=None):
     return device
 
 
+def _overlap(x, y):
+    """Whether the memory that two tensors span overlaps."""
+    a, b = x.data_ptr(), y.data_ptr()
+    reach = [sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * t.element_size() for t in (x, y)]
+    return a <= b + reach[1] and b <= a + reach[0]
+
+
 def cache_write(cache, plan, k, v):
     """Write the new tokens' rows ``k``, ``v`` (packed BF16 [N, heads, D]) to their places.
 
@@ -188,7 +198,7 @@ def _write(cache, plan, k, v):
     index = k.device.index
     sk, sv = k.stride(), v.stride()
     rc = _lib.load().solattn_cache_write(
-        k.data_ptr(), v.data_ptr(), N, H, D, sk[0], sk[1], sv[0], sv[1], *cache._args, *plan._args,
+        k.data_ptr(), v.data_ptr(), N, H, D, sk[0], sk[1], sv[0], sv[1], *cache._args(), *plan._args(),
         plan.page_table.shape[0], error_word(index), current_stream(index))
     if rc:
         _lib.check(rc, "solattn_cache_write")
@@ -212,7 +222,7 @@ def _read(cache, plan, tokens):
     word = error_word(device.index)
     k = torch.empty((B, tokens, H, D), dtype=torch.bfloat16, device=device)
     v = torch.empty((B, tokens, H, D), dtype=torch.bfloat16, device=device)
-    rc = _lib.load().solattn_cache_read(*cache._args, *plan._args[:3], B, H, D, tokens, k.data_ptr(),
+    rc = _lib.load().solattn_cache_read(*cache._args(), *plan._args()[:3], B, H, D, tokens, k.data_ptr(),
                                         v.data_ptr(), word, current_stream(device.index))
     if rc:
         _lib.check(rc, "solattn_cache_read")
@@ -243,6 +253,8 @@ def paged_attention(q, cache, plan, *, window=None, lookahead=0, sink_tokens=0, 
     if out is not None and (out.dtype != torch.bfloat16 or out.device != device or out.shape != q.shape
                             or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
+    if out is not None and _overlap(q, out):
+        raise ValueError("out must not share memory with Q")
     return on_device(device, _attend, q, cache, plan, rule, scale, out, (N, Hq, Hkv, D, page))
 
 
@@ -259,7 +271,7 @@ def _attend(q, cache, plan, rule, scale, out, shape):
         out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=device)
     sq = q.stride()
     rc = _lib.load().solattn_paged_attention(
-        q.data_ptr(), N, Hq, Hkv, D, sq[0], sq[1], *cache._args, *plan._args, B, plan.most_new, *rule, scale,
+        q.data_ptr(), N, Hq, Hkv, D, sq[0], sq[1], *cache._args(), *plan._args(), B, plan.most_new, *rule, scale,
         fresh, ws, size, out.data_ptr(), word, current_stream(device.index))
     if rc:
         _lib.check(rc, "solattn_paged_attention")

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from helpers import to_device
-from paged_reference import E4M3, E8M0, Sequences, assert_within, attend, quantise, values
+from paged_reference import E4M3, E8M0, Sequences, assert_within, attend, quantise, values, visible
 from sol_attn_b200 import (PagedKVCache, PagedPlan, cache_read, cache_write, dense_attention,
                            paged_attention, window_attention)
 from sol_attn_b200.status import DeviceError, check_device_errors
@@ -16,6 +16,37 @@ pytestmark = pytest.mark.gpu
 RULES = [dict(), dict(lookahead=None), dict(window=1), dict(window=37, sink_tokens=5),
          dict(window=100, lookahead=60, sink_tokens=70), dict(window=16, lookahead=None, sink_tokens=16),
          dict(window=5, sink_tokens=100000)]
+
+
+def _plain_gpu(q, k, v, *, window=None, lookahead=0, sink_tokens=0):
+    """Plain attention in 64 bits on the GPU (larger cases) with the tolerance of paged_reference.attend,
+    whose score errors are bounded by the largest score of the call."""
+    G, D = q.shape[2] // k.shape[2], q.shape[3]
+    n, L = q.shape[1], k.shape[1]
+    m = visible(n, L, window, lookahead, sink_tokens).cuda()
+    out, tol = [], []
+    for h in range(q.shape[2]):
+        kk, vv = k[:, :, h // G].double(), v[:, :, h // G].double()
+        s = torch.einsum("bqd,bkd->bqk", q[:, :, h].double(), kk) * D ** -0.5
+        size = float(torch.einsum("bqd,bkd->bqk", q[:, :, h].double().abs(), kk.abs()).max()) * D ** -0.5
+        w = torch.softmax(s.masked_fill(~m, -math.inf), -1).nan_to_num()
+        err = 2 * (D * 2.0 ** -24 * size + 2.0 ** -21 * (1 + size))
+        o = w @ vv
+        out.append(o)
+        tol.append(2.0 ** -8 * o.abs() + (2.0 ** -8 * 1.01 + err) * (w @ vv.abs()) + 1e-30)
+    return torch.stack(out, 2).cpu(), torch.stack(tol, 2).cpu()
+
+
+@pytest.mark.parametrize("rule", [dict(), dict(lookahead=None), dict(window=700, lookahead=300, sink_tokens=130)])
+@pytest.mark.parametrize("B,Tq,Tk,Hq,Hkv,D", [
+    (2, 3001, 3001, 8, 8, 128), (3, 2000, 4500, 12, 4, 64), (1, 1000, 20000, 16, 8, 128), (1, 5, 30000, 12, 1, 64),
+    (40, 2, 3000, 8, 8, 128),
+])
+def test_window_attention_many_items(B, Tq, Tk, Hq, Hkv, D, rule):
+    """Several items per CTA, whole and split ones, clusters and joined splits."""
+    q, k, v = (x.cuda() for x in _bthd(B, Tq, Tk, Hq, Hkv, D, seed=7))
+    assert_within(window_attention(q, k, v, **rule), *_plain_gpu(q, k, v, **rule))
+    check_device_errors()
 
 
 def _bthd(B, Tq, Tk, Hq, Hkv, D, seed=0):
@@ -355,6 +386,25 @@ def test_streams_and_graphs(new):
     assert not torch.equal(again, first)
     check_device_errors()
     del graphs
+
+
+def test_copies_and_overlaps():
+    """A deep copy of cache and plan is a cache and a plan of its own; out may not lie over Q."""
+    import copy
+    s = Sequences([(2, 40), (1, 9)], heads=2, dim=64, page=16, kind="e4m3")
+    q = s.queries(2, 64).cuda()
+    first = paged_attention(q, s.cache, s.plan)
+    cache, plan = copy.deepcopy(s.cache), copy.deepcopy(s.plan)
+    s.cache.k.view(torch.uint8).zero_()
+    s.plan.key_lengths.zero_()
+    assert torch.equal(paged_attention(q, cache, plan), first)
+    assert not paged_attention(q, s.cache, s.plan).any()  # no keys
+    both = torch.zeros((2 * q.shape[0],) + q.shape[1:], dtype=torch.bfloat16, device="cuda")
+    both[:q.shape[0]] = q
+    with pytest.raises(ValueError, match="share"):
+        paged_attention(both[:3], cache, plan, out=both[1:4])
+    assert torch.equal(paged_attention(both[:3], cache, plan, out=both[3:]), first)
+    check_device_errors()
 
 
 @pytest.mark.parametrize("new", [1, 160])
