@@ -10,9 +10,10 @@
 //   S_0(i) S_1(i) | P_0(i) V  S_0(i+1) | P_1(i) V  S_1(i+1) | ...
 //
 // Warps: 0-3 and 4-7 softmax of stage 0 and 1 (a thread per row), 8 issues the MMAs, 9 loads K and V
-// (TMA; E4M3: bulk copies of codes and scales), 10 completes V tiles (rows behind the last key become
+// (TMA; E4M3: bulk copies of codes and scales), 10 completes V tiles (rows that nobody sees become
 // zeros), 11 finds the items and loads Q; E4M3 has 12-15 besides, which convert codes to BF16 tiles.
-// TMEM (512 columns): S_0, S_1 (128 columns each; P, as BF16 pairs, over the first 64), O_0, O_1.
+// TMEM (512 columns): S_0, S_1 (128 columns each; P, as BF16 pairs, over the first 64), O_0, O_1 (128
+// each).  S of a tile goes over P of the one before: the MMAs of one thread run in the order of issue.
 //
 // Keys that a row does not see have no influence whatever they hold: S is replaced by -inf.  Where V
 // is not finite, P = 0 times V would be NaN; an item whose result is not finite is therefore done
@@ -222,7 +223,7 @@ __device__ __forceinline__ bool find_item(const SeqParams& p, int64_t i, int lan
     it.stage[1].sink = it.stage[1].from = it.stage[1].to = 0;
   }
   const int total = it.all.count();
-  it.splits = r < 0 ? 1 : max(1, min(p.splits, (total + p.unit - 1) / p.unit));
+  it.splits = r < 0 ? 1 : split_count<kKeys>(p, total);
   if (split >= it.splits) return false;
   it.c0 = (int)((int64_t)total * split / it.splits);
   it.c1 = (int)((int64_t)total * (split + 1) / it.splits);

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const int r_base = sq.tile * R, off = sq.L - sq.n;
   const int rows = min(R, sq.n * p.G - r_base);
   const KeyTiles kt = key_tiles<T>(p, sq.L, off + r_base / p.G, off + (r_base + rows - 1) / p.G);
-  const int ns = max(1, min(p.splits, (kt.count() + p.unit - 1) / p.unit));
+  const int ns = split_count<T>(p, kt.count());
   if (ns == 1) return;
   pdl_wait();
   const int64_t unit0 = (int64_t)blockIdx.x * p.splits;

@@ -40,7 +40,7 @@ struct SeqParams {
   int32_t* status;     // device-accessible word (pinned host memory) or nullptr
   int B, N, Hq, Hkv, G, Tq, Tk;  // N: rows of q over all sequences (B * Tq when contiguous)
   int window, ahead, sinks;
-  int slots, splits, unit;  // row tiles over all sequences; splits of a tile; key tiles per split
+  int slots, splits, unit;  // row tiles over all sequences; splits of a tile, each of `unit` keys or more
   int cluster;              // few-rows kernel: the splits of a tile are a cluster
   int first;                // chunk kernel: items (a slot and a K/V head) from this number on are split
   int zero_tail;            // write zeros to the rows behind the last sequence
@@ -176,6 +176,12 @@ __device__ __forceinline__ KeyTiles key_tiles(const SeqParams& p, int L, int p0,
   const int sinks = min(p.sinks, high + 1);
   k.sink = min((sinks + T - 1) / T, k.from);
   return k;
+}
+
+// How many splits a row tile with `tiles` key tiles of T keys has.
+template <int T>
+__device__ __forceinline__ int split_count(const SeqParams& p, int tiles) {
+  return max(1, min(p.splits, (tiles * T + p.unit - 1) / p.unit));
 }
 
 // Page of the key tile at `key` (page sizes are multiples of the callers' pieces).  A page outside

@@ -41,7 +41,7 @@ bool rule_ok(const Rule& r) {
 }
 
 // How a kernel divides a call: tiles of rows (slots, see find_seq), and a tile's keys over `splits` CTAs
-// of at least `unit` key tiles each.
+// of `unit` keys or more each.
 struct Split {
   int64_t slots, splits, unit;
   int64_t first = 0;  // chunk kernel: items before this one are not split
@@ -52,7 +52,7 @@ struct Split {
 // The few-rows kernel: tiles of 8 rows where no sequence has more (half of the softmax of 16), 16 else;
 // units of 256 to 2048 keys, as many as give every SM some 8 CTAs, so that sequences of different
 // lengths even out.
-Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t Tq, int64_t most, int64_t cap,
+Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t most, int64_t cap,
                  bool paged, const Rule& r) {
   Split s;
   const int64_t G = Hq / Hkv;
@@ -63,24 +63,23 @@ Split rows_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64
     const int64_t span = r.window + r.lookahead + r.sinks + 16 + 64;
     if (span < keys) keys = span;
   }
-  const int64_t chunk = D == 64 ? 32 : 16;  // keys of a chunk (rows.cu)
-  const int64_t chunks = cdiv(keys, chunk) + 2;
+  keys += 64;  // (chunks of up to 32 keys at both ends)
   const int64_t tiles = s.slots * Hkv;
-  int64_t unit = cdiv(chunks * tiles, kSms * 2 * 4);
-  if (unit < 256 / chunk) unit = 256 / chunk;
-  if (unit > 2048 / chunk) unit = 2048 / chunk;
-  if (unit < cdiv(chunks, 64)) unit = cdiv(chunks, 64);
+  int64_t unit = cdiv(keys * tiles, kSms * 2 * 4);
+  if (unit < 256) unit = 256;
+  if (unit > 2048) unit = 2048;
+  if (unit < cdiv(keys, 64)) unit = cdiv(keys, 64);
   // Up to 8 splits can be a cluster, which joins them by itself, without workspace and second launch (8 x 16
   // heads, 4160 keys: 18.4 -> 12.8 us).  Only where all of the call's clusters run at once: later ones
   // would wait for room for all their CTAs together (64 sequences: 203 -> 250 us), and not where 8
   // CTAs per tile would leave most SMs idle over long keys.
-  const int64_t eighth = cdiv(chunks, 8);
-  if (tiles * 8 <= kSms * 2 && (tiles * 16 >= kSms || eighth * chunk <= 1024)) {
-    unit = eighth * chunk >= 64 ? eighth : 64 / chunk;
-    s.cluster = chunks > unit;
+  const int64_t eighth = cdiv(keys, 8);
+  if (tiles * 8 <= kSms * 2 && (tiles * 16 >= kSms || eighth <= 1024)) {
+    unit = eighth > 64 ? eighth : 64;
+    s.cluster = keys > unit;
   }
   s.unit = unit;
-  s.splits = cdiv(chunks, unit);
+  s.splits = cdiv(keys, unit);
   return s;
 }
 
@@ -118,7 +117,7 @@ Split chunk_split(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int
       }
     }
   }
-  s.unit = cdiv(tiles, s.splits);
+  s.unit = cdiv(tiles, s.splits) * 128;
   return s;
 }
 
@@ -143,7 +142,7 @@ Choice choose(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   const int64_t mean = paged ? N * G / B : Tq * G;
   c.many = most >= kManyRows;
   c.few = mean < kManyRows;
-  c.rows = rows_split(N, B, Hq, Hkv, D, Tq, c.many ? kManyRows : most, cap, paged, r);
+  c.rows = rows_split(N, B, Hq, Hkv, Tq, c.many ? kManyRows : most, cap, paged, r);
   c.chunk = chunk_split(N, B, Hq, Hkv, Tq, cap, paged, r);
   c.rows_bytes = c.few ? split_bytes(c.rows, c.rows.rows, Hkv, D) : 0;
   c.chunk_bytes = c.many ? split_bytes(c.chunk, 256, Hkv, D) : 0;

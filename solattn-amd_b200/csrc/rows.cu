@@ -11,9 +11,9 @@
 // of S and P.  Long sequences are split over several CTAs (`unit` chunks each).  Up to 8 of them
 // form a cluster and join their results through its shared memory; with more, a second kernel joins them.
 //
-// Keys that a row does not see have no influence whatever they hold: S is replaced by -inf, and a
-// chunk with a non-finite V (where P = 0 times V would be NaN) goes through exact_pv, which adds
-// only what each row sees.
+// Keys that a row does not see have no influence whatever they hold: S is replaced by -inf, and where a
+// result is not finite (P = 0 times a V that is not is NaN) the CTA does its keys again, a chunk with such
+// a V through exact_pv, which adds only what each row sees.
 #include "join.cuh"
 
 namespace solattn {
@@ -26,24 +26,26 @@ constexpr int kScaleSpan = 12;  // and may be 2^12 smaller for a key with a smal
 constexpr int kRowThreads = kWarps * 32;
 
 // R rows of a tile: 8 or 16 (of the 16 rows of an MMA).  A chunk has 16 keys per MMA step, two steps
-// where a step is small, so that what a chunk costs besides its bytes is spread over more of them.
+// where a step is small (64 rows of D = 64 or of codes), so that what a chunk costs besides its bytes is
+// spread over more of them.
 template <int D, int KV, int R>
 struct RowsCfg {
   static constexpr int kElt = KV == kPagedE4m3 ? 1 : 2;
   static constexpr int kRowB = D * kElt;          // bytes of a K or V row
-  static constexpr int kSteps = D == 64 ? 2 : 1;
+  static constexpr int kSteps = kRowB >= 256 ? 1 : 2;
   static constexpr int kChunk = 16 * kSteps;      // keys of a chunk
   static constexpr int kCpr = kRowB / 16;         // 16-byte pieces of a row
   static constexpr int kPart = kChunk * kRowB;    // K or V of a chunk
   static constexpr int kStage = 2 * kPart + (KV == kPagedE4m3 ? 2 * kChunk : 0);  // + K and V scales
-  // BF16: 24 KB of ring per warp and two CTAs per SM (the bytes in flight are what counts); E4M3, which
-  // also has codes to convert: three or four CTAs, as many as the registers allow.
-  static constexpr int kStages = KV == kPagedE4m3 && D == 128 ? 4 : 3;
+  // BF16: 24 KB of ring per warp and two CTAs per SM (the bytes in flight are what counts; 6.6 TB/s).
+  // E4M3, which also has codes to convert, wants warps: three CTAs of two stages with D = 128 (6.1 TB/s;
+  // chunks of 16 keys and four stages 5.3), four of three with D = 64 (5.0 TB/s; two or three stages and
+  // other counts of CTAs 4.2 to 5.0).
+  static constexpr int kStages = KV == kPagedE4m3 && D == 128 ? 2 : 3;
   static constexpr int kCtas = KV != kPagedE4m3 ? 2 : D == 64 ? 4 : 3;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kMerge = kWarps * R * (D + 2) * 4;  // m, l, O of every warp
-  static constexpr int kSmem = kWarps * kRing;
-  static_assert(kSmem >= kMerge + R * (D + 2) * 4, "the results of the warps, and of the CTA, over the rings");
+  static constexpr int kSmem = kWarps * kRing > kMerge + R * (D + 2) * 4 ? kWarps * kRing : kMerge + R * (D + 2) * 4;
   static constexpr int kHalves = R / 8;  // row groups g and g + 8 of the MMA
 };
 
@@ -223,7 +225,7 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
   const int pos0 = off + r_base / p.G, pos1 = off + (r_base + rows - 1) / p.G;
   const KeyTiles kt = key_tiles<C::kChunk>(p, sq.L, pos0, pos1);
   const int total = kt.count();
-  const int ns = max(1, min(p.splits, (total + p.unit - 1) / p.unit));
+  const int ns = split_count<C::kChunk>(p, total);
   if (split >= ns) {
     if (p.cluster) {  // (its cluster waits for it twice)
       cluster_sync();
@@ -295,12 +297,15 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
         cp_async16(st + 2 * C::kPart + C::kChunk * lane + 16 * u, (lane ? p.v_scale : p.k_scale) + row0, 16);
     }
   };
-  fetch_pages(0);
+  auto begin = [&]() {
+    fetch_pages(0);
 #pragma unroll
-  for (int i = 0; i < C::kStages - 1; ++i) {
-    if (i < mine) load(i);
-    cp_async_commit();
-  }
+    for (int i = 0; i < C::kStages - 1; ++i) {
+      if (i < mine) load(i);
+      cp_async_commit();
+    }
+  };
+  begin();
 
   // Q fragments: the contraction order over the head dim is free, so lane t of a row group holds the
   // dims that its 16-byte K reads deliver: k-step ks takes 4 consecutive dims of piece 4 (ks / S) + t.
@@ -361,207 +366,223 @@ __global__ void __launch_bounds__(kRowThreads, RowsCfg<D, KV, R>::kCtas) rows_ke
   const int all_hi = key_high(p, sq.L, pos0), all_lo = key_low(p, pos1);  // what every row sees
 
   float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[C::kHalves], l[C::kHalves];
-#pragma unroll
-  for (int half = 0; half < C::kHalves; ++half) {
-    m[half] = -INFINITY;
-    l[half] = 0.f;
-  }
-
-  int ref = 0;  // E4M3: O's scale, as an E8M0 exponent
-
+  int ref;  // E4M3: O's scale, as an E8M0 exponent
+  bool careful = false;
 #pragma unroll 1
-  for (int i = 0; i < mine; ++i) {
-    cp_async_wait<C::kStages - 2>();
-    __syncwarp();  // every lane's pieces of chunk i have landed, and chunk i - 1 has been read
-    const int ahead = i + C::kStages - 1;
-    if (ahead < mine) {
-      if (ahead % kAhead == 0) fetch_pages(ahead);
-      load(ahead);
+  while (true) {  // (a second pass only where a result is not finite)
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int half = 0; half < C::kHalves; ++half) {
+      m[half] = -INFINITY;
+      l[half] = 0.f;
     }
-    cp_async_commit();
-    const int key0 = C::kChunk * kt.at(c0 + warp + i * kWarps);
-    const uint32_t st = ring + (uint32_t)((i % C::kStages) * C::kStage);
-    const uint32_t sv = st + C::kPart;
+    ref = 0;
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      cp_async_wait<C::kStages - 2>();
+      __syncwarp();  // every lane's pieces of chunk i have landed, and chunk i - 1 has been read
+      const int ahead = i + C::kStages - 1;
+      if (ahead < mine) {
+        if (ahead % kAhead == 0) fetch_pages(ahead);
+        load(ahead);
+      }
+      cp_async_commit();
+      const int key0 = C::kChunk * kt.at(c0 + warp + i * kWarps);
+      const uint32_t st = ring + (uint32_t)((i % C::kStages) * C::kStage);
+      const uint32_t sv = st + C::kPart;
 
-    // ---- S = Q K^T: 16 rows, tiles of 8 keys
-    float s[kNt][4];
+      // ---- S = Q K^T: 16 rows, tiles of 8 keys
+      float s[kNt][4];
 #pragma unroll
-    for (int nt = 0; nt < kNt; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int nt = 0; nt < kNt; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
 #pragma unroll
-    for (int hh = 0; hh < C::kCpr / 4; ++hh) {
+      for (int hh = 0; hh < C::kCpr / 4; ++hh) {
 #pragma unroll
-      for (int nt = 0; nt < kNt; ++nt) {
-        const uint4 w4 = lds128(st + k_off<D, KV>(key_of<KV>(nt, g >> 1, g & 1), 4 * hh + t));
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-        if (KV == kPagedE4m3) {
+        for (int nt = 0; nt < kNt; ++nt) {
+          const uint4 w4 = lds128(st + k_off<D, KV>(key_of<KV>(nt, g >> 1, g & 1), 4 * hh + t));
+          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          if (KV == kPagedE4m3) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            mma_f16_16816(s[nt], qa[4 * hh + x], codes_to_f16(w[x], 0), codes_to_f16(w[x], 1));
-        } else {
-          mma_bf16_16816(s[nt], qa[2 * hh], w[0], w[1]);
-          mma_bf16_16816(s[nt], qa[2 * hh + 1], w[2], w[3]);
-        }
-      }
-    }
-    const bool full = key0 + C::kChunk - 1 <= all_hi && (key0 >= all_lo || key0 + C::kChunk <= p.sinks);
-    // E4M3 scales: lane l has those of key l; each lane takes its columns'.  P V runs on FP16 too: P is
-    // multiplied by 2^13 and by the key's V scale relative to `ref`, the largest scale seen so far, to
-    // which O is relative as well.  FP16 then holds every P that matters (down to 2^-37 of the largest
-    // for keys at `ref`, 2^-25 for keys 2^12 below); a chunk with a scale that is further below, or NaN,
-    // goes through exact_pv.  Scales of keys that nobody sees do not count, nor do those of 2^-127
-    // (rows of zeros, or of values below 2^-118).
-    float vs[kNt][2];
-    bool odd_scale = false;
-    if (KV == kPagedE4m3) {
-      const int key = lane & (C::kChunk - 1);
-      const float ks_l = e8m0_value(lds8(st + 2 * C::kPart + key));
-      int e = (int)lds8(st + 2 * C::kPart + C::kChunk + key);
-      if (!full && (key0 + key > high || (key0 + key < low && key0 + key >= p.sinks))) e = 0;
-      odd_scale = __any_sync(0xffffffffu, e == 255);
-      if (e == 255) e = 0;
-      const int most = __reduce_max_sync(0xffffffffu, e);
-      const int least = __reduce_min_sync(0xffffffffu, e == 0 ? 255 : e);
-      if (most > ref) {
-        const float f = two_to(ref - most);
-        ref = most;
-#pragma unroll
-        for (int x = 0; x < D / 8; ++x)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[x][c] *= f;
-      }
-      odd_scale = odd_scale || least < ref - kScaleSpan;
-      const float vs_l = e == 0 ? 0.f : two_to(e - ref + kScaleRoom);
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float f = __shfl_sync(0xffffffffu, ks_l, key_of<KV>(nt, t, c));
-          vs[nt][c] = __shfl_sync(0xffffffffu, vs_l, key_of<KV>(nt, t, c));
-#pragma unroll
-          for (int half = 0; half < C::kHalves; ++half) s[nt][2 * half + c] *= f;
-        }
-    }
-    // ---- visibility
-    bool vis[kNt][4];
-#pragma unroll
-    for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) vis[nt][c] = true;
-    if (!full) {
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2 * C::kHalves; ++c) {
-          const int key = key0 + key_of<KV>(nt, t, c & 1), half = c >> 1;
-          vis[nt][c] = key <= hi[half] && (key >= lo[half] || key < p.sinks);
-          if (!vis[nt][c]) s[nt][c] = -INFINITY;
-        }
-    }
-    // ---- online softmax.  The running maximum moves only when it grows by more than 8 (a factor
-    // 256), so that O is rarely rescaled; P stays at most 256.  (E4M3: 2, for FP16's sake.)
-    float al[2] = {1.f, 1.f};
-    bool need = false;
-#pragma unroll
-    for (int half = 0; half < C::kHalves; ++half) {
-      float x = fmaxf(s[0][2 * half], s[0][2 * half + 1]);
-#pragma unroll
-      for (int nt = 1; nt < kNt; ++nt) x = fmaxf(x, fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * qf[half];
-      if (m[half] == -INFINITY) {
-        m[half] = fmaxf(m[half], x);  // nothing accumulated yet
-      } else if (x > m[half] + (KV == kPagedE4m3 ? 2.f : 8.f)) {
-        al[half] = fast_exp2(m[half] - x);
-        m[half] = x;
-        need = true;
-      }
-    }
-    if (__any_sync(0xffffffffu, need)) {
-#pragma unroll
-      for (int x = 0; x < D / 8; ++x) {
-        o[x][0] *= al[0];
-        o[x][1] *= al[0];
-        o[x][2] *= al[1];
-        o[x][3] *= al[1];
-      }
-#pragma unroll
-      for (int half = 0; half < C::kHalves; ++half) l[half] *= al[half];
-    }
-    float pr[kNt][4];
-#pragma unroll
-    for (int half = 0; half < C::kHalves; ++half) {
-      const float mm = m[half] == -INFINITY ? 0.f : m[half];
-#pragma unroll
-      for (int nt = 0; nt < kNt; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          pr[nt][2 * half + c] = fast_exp2(fmaf(s[nt][2 * half + c], qf[half], -mm));
-          l[half] += pr[nt][2 * half + c];
-        }
-    }
-    // P as the A operand: rounded to BF16 (relative error at most 2^-8 each; l keeps FP32), or, with its
-    // scale, to FP16 (2^-11).
-    uint32_t pa[C::kSteps][4];
-    auto pack = [&](float a, float b) {
-      if (KV != kPagedE4m3) return pack_bf16(a, b);
-      const __half2 y = __floats2half2_rn(a, b);
-      return *reinterpret_cast<const uint32_t*>(&y);
-    };
-#pragma unroll
-    for (int nt = 0; nt < kNt; ++nt) {
-      const float f0 = KV == kPagedE4m3 ? vs[nt][0] : 1.f, f1 = KV == kPagedE4m3 ? vs[nt][1] : 1.f;
-      pa[nt >> 1][2 * (nt & 1)] = pack(pr[nt][0] * f0, pr[nt][1] * f1);
-      pa[nt >> 1][2 * (nt & 1) + 1] = R == 16 ? pack(pr[nt][2] * f0, pr[nt][3] * f1) : 0u;
-    }
-    // ---- O += P V, once V is known to be finite (V * 0 summed is NaN where it is not)
-    uint32_t vb[C::kSteps][D / 8][2];
-    uint32_t acc = 0u;
-#pragma unroll
-    for (int u = 0; u < C::kSteps; ++u) {
-      if (KV == kPagedE4m3) {
-#pragma unroll
-        for (int dd = 0; dd < D / 32; ++dd) {
-          uint32_t w[4];
-          ldsm_codes_t(sv + v_off<D, KV>(16 * u + (lane & 15), 2 * dd + (lane >> 4)), w);
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              vb[u][4 * dd + x][y] = codes_to_f16(w[x], y);
-              acc = f16x2_fma(vb[u][4 * dd + x][y], 0u, acc);
-            }
-        }
-      } else {
-#pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-          ldsm_x4_t(sv + v_off<D, KV>(16 * u + (lane & 15), 2 * dt + (lane >> 4)), vb[u][2 * dt][0],
-                    vb[u][2 * dt][1], vb[u][2 * dt + 1][0], vb[u][2 * dt + 1][1]);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            acc = bf16x2_fma(vb[u][2 * dt + x][0], 0u, acc);
-            acc = bf16x2_fma(vb[u][2 * dt + x][1], 0u, acc);
+            for (int x = 0; x < 4; ++x)
+              mma_f16_16816(s[nt], qa[4 * hh + x], codes_to_f16(w[x], 0), codes_to_f16(w[x], 1));
+          } else {
+            mma_bf16_16816(s[nt], qa[2 * hh], w[0], w[1]);
+            mma_bf16_16816(s[nt], qa[2 * hh + 1], w[2], w[3]);
           }
         }
       }
-    }
-    const bool bad = (acc & 0x7fff7fffu) != 0u || odd_scale;
-    if (__any_sync(0xffffffffu, bad)) {
-      exact_pv<D, KV, R>(o, pr, vis, sv, st + 2 * C::kPart + C::kChunk, ref, lane);
-    } else {
+      const bool full = key0 + C::kChunk - 1 <= all_hi && (key0 >= all_lo || key0 + C::kChunk <= p.sinks);
+      // E4M3 scales: lane l has those of key l; each lane takes its columns'.  P V runs on FP16 too: P is
+      // multiplied by 2^13 and by the key's V scale relative to `ref`, the largest scale seen so far, to
+      // which O is relative as well.  FP16 then holds every P that matters (down to 2^-37 of the largest
+      // for keys at `ref`, 2^-25 for keys 2^12 below); a chunk with a scale that is further below, or NaN,
+      // goes through exact_pv.  Scales of keys that nobody sees do not count, nor do those of 2^-127
+      // (rows of zeros, or of values below 2^-118).
+      float vs[kNt][2];
+      bool odd_scale = false;
+      if (KV == kPagedE4m3) {
+        const int key = lane & (C::kChunk - 1);
+        const float ks_l = e8m0_value(lds8(st + 2 * C::kPart + key));
+        int e = (int)lds8(st + 2 * C::kPart + C::kChunk + key);
+        if (!full && (key0 + key > high || (key0 + key < low && key0 + key >= p.sinks))) e = 0;
+        odd_scale = __any_sync(0xffffffffu, e == 255);
+        if (e == 255) e = 0;
+        const int most = __reduce_max_sync(0xffffffffu, e);
+        const int least = __reduce_min_sync(0xffffffffu, e == 0 ? 255 : e);
+        if (most > ref) {
+          const float f = two_to(ref - most);
+          ref = most;
 #pragma unroll
-      for (int u = 0; u < C::kSteps; ++u)
+          for (int x = 0; x < D / 8; ++x)
 #pragma unroll
-        for (int nt = 0; nt < D / 8; ++nt) {
-          if (KV == kPagedE4m3) mma_f16_16816(o[nt], pa[u], vb[u][nt][0], vb[u][nt][1]);
-          else mma_bf16_16816(o[nt], pa[u], vb[u][nt][0], vb[u][nt][1]);
+            for (int c = 0; c < 4; ++c) o[x][c] *= f;
         }
+        odd_scale = odd_scale || least < ref - kScaleSpan;
+        const float vs_l = e == 0 ? 0.f : two_to(e - ref + kScaleRoom);
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float f = __shfl_sync(0xffffffffu, ks_l, key_of<KV>(nt, t, c));
+            vs[nt][c] = __shfl_sync(0xffffffffu, vs_l, key_of<KV>(nt, t, c));
+#pragma unroll
+            for (int half = 0; half < C::kHalves; ++half) s[nt][2 * half + c] *= f;
+          }
+      }
+      // ---- visibility
+      bool vis[kNt][4];
+#pragma unroll
+      for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vis[nt][c] = true;
+      if (!full) {
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2 * C::kHalves; ++c) {
+            const int key = key0 + key_of<KV>(nt, t, c & 1), half = c >> 1;
+            vis[nt][c] = key <= hi[half] && (key >= lo[half] || key < p.sinks);
+            if (!vis[nt][c]) s[nt][c] = -INFINITY;
+          }
+      }
+      // ---- online softmax.  The running maximum moves only when it grows by more than 8 (a factor
+      // 256), so that O is rarely rescaled; P stays at most 256.  (E4M3: 2, for FP16's sake.)
+      float al[2] = {1.f, 1.f};
+      bool need = false;
+#pragma unroll
+      for (int half = 0; half < C::kHalves; ++half) {
+        float x = fmaxf(s[0][2 * half], s[0][2 * half + 1]);
+#pragma unroll
+        for (int nt = 1; nt < kNt; ++nt) x = fmaxf(x, fmaxf(s[nt][2 * half], s[nt][2 * half + 1]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2)) * qf[half];
+        if (m[half] == -INFINITY) {
+          m[half] = fmaxf(m[half], x);  // nothing accumulated yet
+        } else if (x > m[half] + (KV == kPagedE4m3 ? 2.f : 8.f)) {
+          al[half] = fast_exp2(m[half] - x);
+          m[half] = x;
+          need = true;
+        }
+      }
+      if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          o[x][0] *= al[0];
+          o[x][1] *= al[0];
+          o[x][2] *= al[1];
+          o[x][3] *= al[1];
+        }
+#pragma unroll
+        for (int half = 0; half < C::kHalves; ++half) l[half] *= al[half];
+      }
+      float pr[kNt][4];
+#pragma unroll
+      for (int half = 0; half < C::kHalves; ++half) {
+        const float mm = m[half] == -INFINITY ? 0.f : m[half];
+#pragma unroll
+        for (int nt = 0; nt < kNt; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            pr[nt][2 * half + c] = fast_exp2(fmaf(s[nt][2 * half + c], qf[half], -mm));
+            l[half] += pr[nt][2 * half + c];
+          }
+      }
+      // P as the A operand: rounded to BF16 (relative error at most 2^-8 each; l keeps FP32), or, with its
+      // scale, to FP16 (2^-11).
+      uint32_t pa[C::kSteps][4];
+      auto pack = [&](float a, float b) {
+        if (KV != kPagedE4m3) return pack_bf16(a, b);
+        const __half2 y = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&y);
+      };
+#pragma unroll
+      for (int nt = 0; nt < kNt; ++nt) {
+        const float f0 = KV == kPagedE4m3 ? vs[nt][0] : 1.f, f1 = KV == kPagedE4m3 ? vs[nt][1] : 1.f;
+        pa[nt >> 1][2 * (nt & 1)] = pack(pr[nt][0] * f0, pr[nt][1] * f1);
+        pa[nt >> 1][2 * (nt & 1) + 1] = R == 16 ? pack(pr[nt][2] * f0, pr[nt][3] * f1) : 0u;
+      }
+      // ---- O += P V.  P = 0 times a V that is not finite would be NaN: the first pass takes the chance, and
+      // a result that is not finite is done again, each chunk's V being looked at first.
+      auto v_step = [&](int u, int dd, uint32_t (&vb)[4][2]) {  // dims 32 dd .. of 16 keys
+        if (KV == kPagedE4m3) {
+          uint32_t w[4];
+          ldsm_codes_t(sv + v_off<D, KV>(16 * u + (lane & 15), 2 * dd + (lane >> 4)), w);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            vb[x][0] = codes_to_f16(w[x], 0);
+            vb[x][1] = codes_to_f16(w[x], 1);
+          }
+        } else {
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            ldsm_x4_t(sv + v_off<D, KV>(16 * u + (lane & 15), 4 * dd + 2 * y + (lane >> 4)), vb[2 * y][0], vb[2 * y][1],
+                      vb[2 * y + 1][0], vb[2 * y + 1][1]);
+        }
+      };
+      bool exact = odd_scale;
+      if (careful) {
+        uint32_t acc = 0u;  // V * 0 summed: NaN where a V is not finite
+#pragma unroll 1
+        for (int u = 0; u < C::kSteps; ++u)
+#pragma unroll 1
+          for (int dd = 0; dd < D / 32; ++dd) {
+            uint32_t vb[4][2];
+            v_step(u, dd, vb);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              acc = KV == kPagedE4m3 ? f16x2_fma(vb[x >> 1][x & 1], 0u, acc) : bf16x2_fma(vb[x >> 1][x & 1], 0u, acc);
+          }
+        exact = exact || __any_sync(0xffffffffu, (acc & 0x7fff7fffu) != 0u);
+      }
+      if (exact) {
+        exact_pv<D, KV, R>(o, pr, vis, sv, st + 2 * C::kPart + C::kChunk, ref, lane);
+      } else {
+#pragma unroll
+        for (int u = 0; u < C::kSteps; ++u)
+#pragma unroll
+          for (int dd = 0; dd < D / 32; ++dd) {
+            uint32_t vb[4][2];
+            v_step(u, dd, vb);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if (KV == kPagedE4m3) mma_f16_16816(o[4 * dd + x], pa[u], vb[x][0], vb[x][1]);
+              else mma_bf16_16816(o[4 * dd + x], pa[u], vb[x][0], vb[x][1]);
+            }
+          }
+      }
     }
+    cp_async_wait<0>();
+    float check = 0.f;  // not zero where a result is not finite
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+      for (int c = 0; c < 2 * C::kHalves; ++c) check = fmaf(o[i][c], 0.f, check);
+    if (!__syncthreads_or(check != 0.f) || careful) break;
+    careful = true;
+    begin();
   }
-  cp_async_wait<0>();
-  __syncthreads();
 
   // ---- the warps' results through shared memory (over the rings, which are drained)
   float* sO = reinterpret_cast<float*>(smem);  // [warp][row][D]
