@@ -1071,7 +1071,7 @@ cudaError_t launch_chunk_kv(const SeqParams& p, cudaStream_t stream) {
   kernel<<<(unsigned)(units < sms ? units : sms), C::kThreads, C::kBytes, stream>>>(p, tmK, tmV);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1 || split_items == 0) return err;
-  return launch_join<D, kItemRows, kKeys>(p, dim3((unsigned)split_items, kItemRows / 16), stream);
+  return launch_join<D, kItemRows, kKeys>(p, split_items, stream);
 }
 
 }  // namespace

@@ -11,8 +11,8 @@ constexpr int kJoinThreads = 128;
 
 // out = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - max m), over a row's partial results: O at
 // part[unit][R][D], m and l behind all of them.  R rows of a tile, T keys of a key tile, as in the
-// kernel that wrote them.  A CTA takes 16 rows of a tile, a warp one row at a time; the order over
-// the splits is fixed, so that a call gives the same bits each time.
+// kernel that wrote them.  A warp takes a row; the order over the splits (at most 64) is fixed, so that a
+// call gives the same bits each time.
 template <int D, int R, int T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -34,44 +34,64 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const SeqParams p) {
   const int64_t unit0 = (int64_t)blockIdx.x * p.splits;
   const float2* ml0 = reinterpret_cast<const float2*>(p.part + (int64_t)gridDim.x * p.splits * R * D);
   constexpr int kPer = D / 32;  // dims of a lane
-  const int r0 = 16 * blockIdx.y, r1 = min(rows, r0 + 16);
-  for (int r = r0 + warp; r < r1; r += kJoinThreads / 32) {
-    float mx = -INFINITY;
-    for (int s = lane; s < ns; s += 32) mx = fmaxf(mx, ml0[(unit0 + s) * R + r].x);
+  const int r = (kJoinThreads / 32) * blockIdx.y + warp;
+  if (r >= rows) return;
+  // Lane l has m and l of splits l, l + 32 (of at most 64), then their weights.
+  float m[2], l[2], mx = -INFINITY;
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f, a[kPer];
-#pragma unroll
-    for (int x = 0; x < kPer; ++x) a[x] = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < ns; ++s) {
-      const float2 ml = ml0[(unit0 + s) * R + r];
-      const float f = fast_exp2(ml.x - base);
-      sum += ml.y * f;
-      const float* src = p.part + ((unit0 + s) * R + r) * D + kPer * lane;
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) a[x] += src[x] * f;
-    }
-    const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
-    const int high = key_high(p, sq.L, pos);
-    const bool any = high >= 0 && (high >= key_low(p, pos) || p.sinks > 0);
-    const float inv = any ? 1.f / sum : 0.f;
-    __nv_bfloat16* dst = p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + kPer * lane;
-#pragma unroll
-    for (int x = 0; x < kPer; x += 2)
-      *reinterpret_cast<uint32_t*>(dst + x) = any ? pack_bf16(a[x] * inv, a[x + 1] * inv) : 0u;
+  for (int x = 0; x < 2; ++x) {
+    const int s = lane + 32 * x;
+    const float2 ml = s < ns ? ml0[(unit0 + s) * R + r] : make_float2(-INFINITY, 0.f);
+    m[x] = ml.x;
+    l[x] = ml.y;
+    mx = fmaxf(mx, ml.x);
   }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f, a[kPer];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    m[x] = fast_exp2(m[x] - base);
+    sum += l[x] * m[x];
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+#pragma unroll
+  for (int x = 0; x < kPer; ++x) a[x] = 0.f;
+  const float* src = p.part + (unit0 * R + r) * D + kPer * lane;
+#pragma unroll 8
+  for (int s = 0; s < ns; ++s) {
+    const float f = __shfl_sync(0xffffffffu, s < 32 ? m[0] : m[1], s & 31);
+    float v[kPer];
+    if (kPer == 4) {
+      const float4 v4 = *reinterpret_cast<const float4*>(src + (int64_t)s * R * D);
+      v[0] = v4.x, v[1] = v4.y, v[kPer - 2] = v4.z, v[kPer - 1] = v4.w;
+    } else {
+      const float2 v2 = *reinterpret_cast<const float2*>(src + (int64_t)s * R * D);
+      v[0] = v2.x, v[1] = v2.y;
+    }
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) a[x] += v[x] * f;
+  }
+  const int tok = (r_base + r) / p.G, head = (r_base + r) % p.G, pos = off + tok;
+  const int high = key_high(p, sq.L, pos);
+  const bool any = high >= 0 && (high >= key_low(p, pos) || p.sinks > 0);
+  const float inv = any ? 1.f / sum : 0.f;
+  __nv_bfloat16* dst = p.out + ((int64_t)(sq.start + tok) * p.Hq + h * p.G + head) * D + kPer * lane;
+#pragma unroll
+  for (int x = 0; x < kPer; x += 2)
+    *reinterpret_cast<uint32_t*>(dst + x) = any ? pack_bf16(a[x] * inv, a[x + 1] * inv) : 0u;
 }
 
-// Launches the join behind the kernel that was launched last on `stream`.
+// Launches the join of `tiles` row tiles behind the kernel that was launched last on `stream`.
 template <int D, int R, int T>
-cudaError_t launch_join(const SeqParams& p, dim3 grid, cudaStream_t stream) {
+cudaError_t launch_join(const SeqParams& p, int64_t tiles, cudaStream_t stream) {
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((unsigned)tiles, R / (kJoinThreads / 32));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cfg.attrs = &attr;

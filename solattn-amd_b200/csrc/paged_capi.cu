@@ -126,9 +126,12 @@ int64_t split_bytes(const Split& s, int64_t tile_rows, int64_t Hkv, int64_t D) {
 }
 
 // Which kernels a call takes.  The few-rows kernel reads its keys once per 16 rows, the chunk kernel
-// once per 256 but with tiles that are mostly empty for few rows; they meet at about kManyRows rows
-// of a sequence.  A packed call whose sequences may lie on both sides launches both, each for its own.
-constexpr int64_t kManyRows = 64;
+// once per 256 but with tiles that are mostly empty for few rows.  Measured, few-rows / chunk: 8 ragged
+// sequences up to 8192 keys, 8 heads, D 128, up to 96 new tokens 91 / 97 us (BF16) and 83 / 128 us
+// (E4M3), up to 128 tokens 114 / 97 and 116 / 127; 32 sequences of 2000 keys, 96 tokens 90 / 84; one of
+// 4000 keys, 4 heads, 128 tokens 16 / 21, 256 tokens 38 / 24.  A packed call whose sequences may lie on
+// both sides launches both, each for its own.
+constexpr int64_t kManyRows = 96;
 struct Choice {
   bool few, many;
   Split rows, chunk;

@@ -709,7 +709,7 @@ cudaError_t launch_rows_kv(const SeqParams& p, cudaStream_t stream) {
   rows_kernel<D, KV, R><<<(unsigned)(tiles * p.splits), kRowThreads, C::kSmem, stream>>>(p);
   err = cudaGetLastError();
   if (err != cudaSuccess || p.splits == 1) return err;
-  return launch_join<D, R, C::kChunk>(p, dim3((unsigned)tiles), stream);
+  return launch_join<D, R, C::kChunk>(p, tiles, stream);
 }
 
 template <int D, int R>
