@@ -1,7 +1,7 @@
 // Writing new tokens' K/V rows into a paged cache and reading sequences back.
 //
-// Both are copies, bound by HBM bandwidth: a row of D values of one (token, head) is handled by D / 8
-// lanes, each with 16 bytes of BF16.  E4M3 rows get one power-of-two scale: e is the least integer
+// Both are copies, bound by HBM bandwidth once the instructions around a row are few: a row of D values
+// of one (token, head) is handled by D / 8 lanes (16 bytes of BF16 each; reading) or D / 16 (writing).  E4M3 rows get one power-of-two scale: e is the least integer
 // with max|x| <= 448 * 2^e (448 is the largest E4M3 value), so x * 2^-e is exact and the conversion
 // rounds once; E4M3 is itself a floating format, so a power of two as the scale costs no precision
 // against max|x| / 448.  A value that is not finite does not enter the maximum; infinities become
@@ -15,7 +15,9 @@ namespace solattn {
 namespace {
 
 constexpr int kCopyThreads = 256;
-constexpr int kRun = 4;  // rows of a group of lanes (read of 32768 x 24 E4M3 rows: 1, 2, 4: 147, 110, 95 us)
+// Rows of a group of lanes.  E4M3 prompt of 23616 x 24 x 128 written, 1, 2, 4 rows: 74, 69, 68 us (6.4 TB/s; a
+// decoding step's 512 rows 2.9, 3.1, 3.7 us); 32768 x 24 x 128 read, 1, 2, 4: 147, 110, 94 us (6.4 TB/s).
+constexpr int kWriteRun = 2, kRun = 4;
 
 // 448 * 2^e >= top for the least e, as the biased exponent e + 127 clamped to [0, 254]: with top =
 // f * 2^x, 1 <= f < 2, that is x - 8 where f <= 1.75, else x - 7.
@@ -49,22 +51,26 @@ __device__ __forceinline__ int seq_of_token(const CacheParams& p, int tok) {
 
 }  // namespace
 
-// kRun consecutive rows (token, head) of K or V per group of D / 8 lanes, all loads before the first store.
+// kRun consecutive rows (token, head) of K or V per group of D / 16 lanes (32 bytes each: what a row
+// costs besides its bytes is shared by fewer lanes), all loads before the first store.
 template <int D, bool kE4m3>
 __global__ void __launch_bounds__(kCopyThreads) cache_write_kernel(const CacheParams p) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   const int sub = threadIdx.x % kLanes, z = blockIdx.y;
   const uint32_t rows = (uint32_t)p.N * (uint32_t)p.Hkv;  // (below 2^31: checked by the host)
-  const uint32_t row0 = (blockIdx.x * (uint32_t)(kCopyThreads / kLanes) + threadIdx.x / kLanes) * kRun;
+  const uint32_t row0 = (blockIdx.x * (uint32_t)(kCopyThreads / kLanes) + threadIdx.x / kLanes) * kWriteRun;
   const uint32_t first = min(row0, rows - 1);
   const int tok0 = (int)(first / (uint32_t)p.Hkv), h0 = (int)(first % (uint32_t)p.Hkv);
-  uint4 raw[kRun];
+  uint4 raw[kWriteRun][2];
   int tok = tok0, h = h0;
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
-    raw[j] = make_uint4(0, 0, 0, 0);
-    if (row0 + j < rows)
-      raw[j] = __ldg(reinterpret_cast<const uint4*>(p.x[z] + (int64_t)tok * p.sT[z] + (int64_t)h * p.sH[z]) + sub);
+  for (int j = 0; j < kWriteRun; ++j) {
+    raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
+    if (row0 + j < rows) {
+      const uint4* src = reinterpret_cast<const uint4*>(p.x[z] + (int64_t)tok * p.sT[z] + (int64_t)h * p.sH[z]) + 2 * sub;
+      raw[j][0] = __ldg(src);
+      raw[j][1] = __ldg(src + 1);
+    }
     if (++h == p.Hkv) {
       h = 0;
       ++tok;
@@ -72,13 +78,13 @@ __global__ void __launch_bounds__(kCopyThreads) cache_write_kernel(const CachePa
   }
   // Their places in the cache (rows of it), or -1.  The heads of a token are a page's rows apart, so
   // that the token is looked up once.
-  int64_t dst[kRun];
+  int64_t dst[kWriteRun];
   int start = 0, next = 0, last = 0, b = -1;  // the token's sequence: its packed tokens, key_lengths - next
   int64_t at = -1;
   tok = tok0;
   h = h0;
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
+  for (int j = 0; j < kWriteRun; ++j) {
     if (row0 + j < rows && (j == 0 || h == 0)) {
       if (b < 0 || tok >= next || tok < start) {
         b = seq_of_token(p, tok);
@@ -105,21 +111,28 @@ __global__ void __launch_bounds__(kCopyThreads) cache_write_kernel(const CachePa
   }
   if constexpr (!kE4m3) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j)
-      if (dst[j] >= 0) reinterpret_cast<uint4*>(p.pages[z] + dst[j] * D * 2)[sub] = raw[j];
+    for (int j = 0; j < kWriteRun; ++j)
+      if (dst[j] >= 0) {
+        uint4* to = reinterpret_cast<uint4*>(p.pages[z] + dst[j] * D * 2) + 2 * sub;
+        to[0] = raw[j][0];
+        to[1] = raw[j][1];
+      }
   } else {
     // The largest magnitude of a row, as BF16 bits (which order like the values), pairs at a time.
-    uint32_t top[kRun];
+    uint32_t top[kWriteRun];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      top[j] = __vimax3_u16x2(raw[j].x & 0x7fff7fffu, raw[j].y & 0x7fff7fffu, raw[j].z & 0x7fff7fffu);
-      top[j] = __vimax3_u16x2(top[j], top[j], raw[j].w & 0x7fff7fffu);
+    for (int j = 0; j < kWriteRun; ++j) {
+      const uint32_t x[8] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w,
+                             raw[j][1].x, raw[j][1].y, raw[j][1].z, raw[j][1].w};
+      top[j] = x[7] & 0x7fff7fffu;
+#pragma unroll
+      for (int i = 0; i < 6; i += 2) top[j] = __vimax3_u16x2(top[j], x[i] & 0x7fff7fffu, x[i + 1] & 0x7fff7fffu);
+      top[j] = __vimax3_u16x2(top[j], top[j], x[6] & 0x7fff7fffu);
       if ((top[j] & 0xffffu) >= 0x7f80u || (top[j] >> 16) >= 0x7f80u) {  // (rare) not finite: left out
-        const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
         top[j] = 0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t m = (w[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t m = (x[i >> 1] >> (16 * (i & 1))) & 0x7fffu;
           if (m < 0x7f80u) top[j] = max(top[j], m);
         }
       }
@@ -127,13 +140,14 @@ __global__ void __launch_bounds__(kCopyThreads) cache_write_kernel(const CachePa
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) top[j] = __vimax3_u16x2(top[j], top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
+      for (int j = 0; j < kWriteRun; ++j) top[j] = __vimax3_u16x2(top[j], top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
+    for (int j = 0; j < kWriteRun; ++j) {
       const int e = scale_exponent(__uint_as_float(max(top[j] & 0xffffu, top[j] >> 16) << 16));
-      const uint2 c = to_e4m3(raw[j], __uint_as_float((uint32_t)(254 - e) << 23));
+      const float f = __uint_as_float((uint32_t)(254 - e) << 23);
+      const uint2 c0 = to_e4m3(raw[j][0], f), c1 = to_e4m3(raw[j][1], f);
       if (dst[j] >= 0) {
-        reinterpret_cast<uint2*>(p.pages[z] + dst[j] * D)[sub] = c;
+        reinterpret_cast<uint4*>(p.pages[z] + dst[j] * D)[sub] = make_uint4(c0.x, c0.y, c1.x, c1.y);
         if (sub == 0) p.scale[z][dst[j]] = (uint8_t)e;
       }
     }
@@ -217,14 +231,14 @@ __global__ void __launch_bounds__(kCopyThreads) cache_read_kernel(const CachePar
   }
 }
 
-// Blocks for `rows` rows.
-static unsigned copy_blocks(int64_t rows, int D) {
-  const int64_t per = (int64_t)(kCopyThreads / (D / 8)) * kRun;
+// Blocks for `rows` rows, of which `lanes` lanes take `run`.
+static unsigned copy_blocks(int64_t rows, int lanes, int run) {
+  const int64_t per = (int64_t)(kCopyThreads / lanes) * run;
   return (unsigned)((rows + per - 1) / per);
 }
 
 cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream) {
-  const dim3 grid(copy_blocks((int64_t)p.N * p.Hkv, D), 2);
+  const dim3 grid(copy_blocks((int64_t)p.N * p.Hkv, D / 16, kWriteRun), 2);
   if (D == 128) {
     if (p.scale[0]) cache_write_kernel<128, true><<<grid, kCopyThreads, 0, stream>>>(p);
     else cache_write_kernel<128, false><<<grid, kCopyThreads, 0, stream>>>(p);
@@ -236,7 +250,7 @@ cudaError_t launch_cache_write(const CacheParams& p, int D, cudaStream_t stream)
 }
 
 cudaError_t launch_cache_read(const CacheParams& p, int D, cudaStream_t stream) {
-  const dim3 grid(copy_blocks((int64_t)p.B * p.tokens * p.Hkv, D), 2);
+  const dim3 grid(copy_blocks((int64_t)p.B * p.tokens * p.Hkv, D / 8, kRun), 2);
   if (D == 128) {
     if (p.scale[0]) cache_read_kernel<128, true><<<grid, kCopyThreads, 0, stream>>>(p);
     else cache_read_kernel<128, false><<<grid, kCopyThreads, 0, stream>>>(p);

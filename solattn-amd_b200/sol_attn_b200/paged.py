@@ -17,7 +17,7 @@ import torch
 from . import _lib
 from .attention import _is_b200, _nonnegative_integer
 from .status import error_word
-from .window import aligned, check_inputs, check_rule, check_scale, current_stream, on_device, workspace
+from .window import check_rule, check_scale, checked, current_stream, on_device, workspace
 
 PAGE_SIZES = (16, 32, 64, 128)
 
@@ -137,21 +137,26 @@ class PagedPlan:
             raise ValueError("PagedPlan.create takes CPU tensors")
         if page_size not in PAGE_SIZES:
             raise ValueError("page_size must be 16, 32, 64 or 128")
-        plan = cls(*(x.clone().contiguous() for x in xs))
-        if int(query_starts[0]) != 0 or bool((query_starts[1:] < query_starts[:-1]).any()):
+        plan = cls(*(x.clone(memory_format=torch.contiguous_format) for x in xs))
+        table, lengths, starts = (x.numpy() for x in (plan.page_table, plan.key_lengths, plan.query_starts))
+        new = starts[1:] - starts[:-1]
+        if starts[0] != 0 or new.min() < 0:
             raise ValueError("query_starts must begin with 0 and not decrease")
-        if bool((key_lengths < 0).any()) or bool((key_lengths > page_table.shape[1] * page_size).any()):
+        if lengths.min() < 0 or lengths.max() > table.shape[1] * page_size:
             raise ValueError("key_lengths must fit in the page table")
-        if bool((query_starts[1:] - query_starts[:-1] > key_lengths).any()):
+        if (new > lengths).any():
             raise ValueError("A sequence has more new tokens than keys")
-        if pages is not None and bool((page_table >= pages).any()):
+        if pages is not None and table.max() >= pages:
             raise ValueError("page_table names a page outside the cache")
-        return cls(plan.page_table, plan.key_lengths, plan.query_starts,
-                   int((query_starts[1:] - query_starts[:-1]).max()))
+        object.__setattr__(plan, "most_new", int(new.max()))
+        return plan
 
     def to(self, device):
-        return PagedPlan(*(x.to(device) for x in (self.page_table, self.key_lengths, self.query_starts)),
-                         self.most_new)
+        """The plan on ``device`` (one transfer)."""
+        t = self.page_table
+        flat = torch.cat((t.reshape(-1), self.key_lengths, self.query_starts)).to(device)
+        n, b = t.numel(), t.shape[0]
+        return PagedPlan(flat[:n].view(t.shape), flat[n:n + b], flat[n + b:], self.most_new)
 
 
 def _check(cache, plan, x=None):
@@ -182,21 +187,19 @@ def cache_write(cache, plan, k, v):
     """
     if k.ndim != 3 or k.shape != v.shape or 0 in k.shape:
         raise ValueError("K/V must have matching nonempty [tokens, heads, D] shapes")
-    check_inputs(k, v)
+    (k, sk), (v, sv) = checked(k), checked(v)
     device = _check(cache, plan, k)
     if v.device != device:
         raise ValueError("The sm_100a backend requires the cache and Q/K/V on the same NVIDIA B200 CUDA GPU")
     pages = cache.k.shape
     if k.shape[1] != pages[1] or k.shape[2] != pages[3]:
         raise ValueError("K/V heads and dimension must match the cache")
-    on_device(device, _write, cache, plan, k, v)
+    on_device(device, _write, cache, plan, k, v, sk, sv)
 
 
-def _write(cache, plan, k, v):
-    k, v = aligned(k), aligned(v)
+def _write(cache, plan, k, v, sk, sv):
     N, H, D = k.shape
     index = k.device.index
-    sk, sv = k.stride(), v.stride()
     rc = _lib.load().solattn_cache_write(
         k.data_ptr(), v.data_ptr(), N, H, D, sk[0], sk[1], sv[0], sv[1], *cache._args(), *plan._args(),
         plan.page_table.shape[0], error_word(index), current_stream(index))
@@ -242,7 +245,7 @@ def paged_attention(q, cache, plan, *, window=None, lookahead=0, sink_tokens=0, 
     """
     if q.ndim != 3 or 0 in q.shape:
         raise ValueError("Q must be a nonempty packed [tokens, heads, D] tensor")
-    check_inputs(q)
+    rows, sq = checked(q)
     device = _check(cache, plan, q)
     N, Hq, D = q.shape
     _, Hkv, page, cache_dim = cache.k.shape
@@ -255,11 +258,10 @@ def paged_attention(q, cache, plan, *, window=None, lookahead=0, sink_tokens=0, 
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
     if out is not None and _overlap(q, out):
         raise ValueError("out must not share memory with Q")
-    return on_device(device, _attend, q, cache, plan, rule, scale, out, (N, Hq, Hkv, D, page))
+    return on_device(device, _attend, rows, sq, cache, plan, rule, scale, out, (N, Hq, Hkv, D, page))
 
 
-def _attend(q, cache, plan, rule, scale, out, shape):
-    q = aligned(q)
+def _attend(q, sq, cache, plan, rule, scale, out, shape):
     N, Hq, Hkv, D, page = shape
     device = q.device
     B, width = plan.page_table.shape
@@ -269,7 +271,6 @@ def _attend(q, cache, plan, rule, scale, out, shape):
     fresh = out is None
     if fresh:
         out = torch.empty((N, Hq, D), dtype=torch.bfloat16, device=device)
-    sq = q.stride()
     rc = _lib.load().solattn_paged_attention(
         q.data_ptr(), N, Hq, Hkv, D, sq[0], sq[1], *cache._args(), *plan._args(), B, plan.most_new, *rule, scale,
         fresh, ws, size, out.data_ptr(), word, current_stream(device.index))

@@ -12,7 +12,7 @@ import math
 import torch
 
 from . import _lib
-from .attention import _aligned, _is_b200
+from .attention import _is_b200
 from .status import error_word
 
 # The current stream's handle without the stream object around it (a third of a small call's cost).
@@ -64,24 +64,26 @@ def workspace(fn, key, device):
     return x, x.data_ptr(), size
 
 
-def aligned(x):
-    """``x``, or a copy, with rows on 16-byte boundaries (a copy also where only the stride of a
-    dimension of size 1 or the start is odd, which ``contiguous`` would leave alone)."""
-    return x if _aligned(x) else x.clone(memory_format=torch.contiguous_format)
-
-
-def check_inputs(*xs):
-    """Checks shared by the inference-only BF16 operators beyond their shapes."""
-    for x in xs:
-        if x.dtype is not torch.bfloat16:
-            raise ValueError("Only BF16 Q/K/V are implemented")
-        if x.requires_grad:
-            raise ValueError("Inference only: Q/K/V must not require gradients")
-        strides = x.stride()
-        if strides[-1] != 1 or min(strides) <= 0:
-            raise ValueError("Q/K/V need positive strides and contiguous head dimension")
-    if xs[0].shape[-1] not in (64, 128):
+def checked(x):
+    """``x`` (or an aligned copy) after the checks that the inference-only BF16 operators share beyond
+    shapes and devices, with its strides.  Rows have to start on 16-byte boundaries; a copy is also made
+    where only the stride of a dimension of size 1 or the start is odd."""
+    if x.dtype is not torch.bfloat16:
+        raise ValueError("Only BF16 Q/K/V are implemented")
+    if x.requires_grad:
+        raise ValueError("Inference only: Q/K/V must not require gradients")
+    strides = x.stride()
+    if strides[-1] != 1 or min(strides) <= 0:
+        raise ValueError("Q/K/V need positive strides and contiguous head dimension")
+    if x.shape[-1] not in (64, 128):
         raise ValueError("Only head dimensions 64 and 128 are implemented")
+    odd = x.data_ptr() & 15
+    for s in strides[:-1]:
+        odd |= s & 7
+    if odd:
+        x = x.clone(memory_format=torch.contiguous_format)
+        strides = x.stride()
+    return x, strides
 
 
 def on_device(device, fn, *args):
@@ -109,26 +111,24 @@ def window_attention(q, k, v, *, window=None, lookahead=0, sink_tokens=0, scale=
     if k.shape != v.shape or B != Bk or D != Dk or 0 in (B, Tq, Hq, D, Tk, Hkv) or Hq % Hkv:
         raise ValueError("Q/K/V batch and dimension shapes must agree and be nonempty, and Q heads "
                          "be a multiple of K/V heads")
-    check_inputs(q, k, v)
+    (q, sq), (k, sk), (v, sv) = checked(q), checked(k), checked(v)
     scale = check_scale(scale, D)
     rule = check_rule(window, lookahead, sink_tokens)
     device = q.device
     if (device.type != "cuda" or k.device != device or v.device != device
             or not _is_b200(device)):
         raise ValueError("The sm_100a backend requires Q/K/V on the same NVIDIA B200 CUDA GPU")
-    return on_device(device, _launch, q, k, v, rule, scale, (B, Tq, Tk, Hq, Hkv, D))
+    return on_device(device, _launch, q, k, v, rule, scale, (B, Tq, Tk, Hq, Hkv, D), sq[:3] + sk[:3] + sv[:3])
 
 
-def _launch(q, k, v, rule, scale, shape):
-    q, k, v = aligned(q), aligned(k), aligned(v)
+def _launch(q, k, v, rule, scale, shape, strides):
     device = q.device
     word = error_word(device.index)  # an earlier call's device-side error surfaces here
     keep, ws, size = workspace("solattn_window_workspace_bytes", shape + rule, device)
     out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
-    sq, sk, sv = q.stride(), k.stride(), v.stride()
     rc = _lib.load().solattn_window_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, sq[0], sq[1], sq[2], sk[0], sk[1], sk[2],
-        sv[0], sv[1], sv[2], *rule, scale, ws, size, out.data_ptr(), word, current_stream(device.index))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, *strides, *rule, scale, ws, size, out.data_ptr(),
+        word, current_stream(device.index))
     if rc:
         _lib.check(rc, "solattn_window_attention")
     return out
