@@ -1,10 +1,10 @@
 // Writing new tokens' K/V rows into a paged cache and reading sequences back.
 //
 // Both are copies, bound by HBM bandwidth once the instructions around a row are few: a row of D values
-// of one (token, head) is handled by D / 8 lanes (16 bytes of BF16 each; reading) or D / 16 (writing).  E4M3 rows get one power-of-two scale: e is the least integer
-// with max|x| <= 448 * 2^e (448 is the largest E4M3 value), so x * 2^-e is exact and the conversion
-// rounds once; E4M3 is itself a floating format, so a power of two as the scale costs no precision
-// against max|x| / 448.  A value that is not finite does not enter the maximum; infinities become
+// of one (token, head) is handled by D / 8 lanes (16 bytes of BF16 each; reading) or D / 16 (writing).
+// E4M3 rows get one power-of-two scale: e is the least integer with max|x| <= 448 * 2^e (448 is the
+// largest E4M3 value), so x * 2^-e is exact and the conversion rounds once; E4M3 is itself a floating
+// format, so a power of two as the scale costs no precision against max|x| / 448.  A value that is not finite does not enter the maximum; infinities become
 // +-448 * 2^e and NaN stays NaN.
 #include <cuda_fp8.h>
 
