@@ -48,10 +48,11 @@ struct ChunkCfg {
   static constexpr bool kCodes = KV == kPagedE4m3;
   static constexpr int kThreads = kCodes ? 512 : 384;
   // Registers: the launch's threads x registers divided between the softmax warpgroups and the rest
-  // (setmaxnreg); the host checks that the kernel was compiled to kLaunchRegs.
+  // (setmaxnreg); the host checks that the kernel was compiled to kLaunchRegs.  9472 tokens over
+  // themselves, 4 heads, BF16: softmax registers 192, 200, 208, 216: 152, 149, 155, 159 us (D 128).
   static constexpr int kLaunchRegs = kCodes ? 128 : 168;
-  static constexpr int kSoftmaxRegs = kCodes ? 184 : 208;
-  static constexpr int kOtherRegs = kCodes ? 72 : 88;
+  static constexpr int kSoftmaxRegs = kCodes ? (D == 128 ? 176 : 184) : 200;
+  static constexpr int kOtherRegs = kCodes ? 256 - kSoftmaxRegs : 104;
   static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in what the launch holds");
   static constexpr int kTile = kKeys * D * 2;  // a K, V or stage's Q tile
