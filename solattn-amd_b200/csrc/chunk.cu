@@ -9,11 +9,16 @@
 //
 //   S_0(i) S_1(i) | P_0(i) V  S_0(i+1) | P_1(i) V  S_1(i+1) | ...
 //
+// A stage waits for its S from the moment it hands P over: about a third of a tile's time.  With D 64
+// BF16, where TMEM holds a third S buffer, S is issued one (tile, stage) pair earlier, and a stage finds
+// its next S ready (9472 tokens over themselves, 4 heads: 138 -> 126 us); the E4M3 converters lose by
+// it (D 64: 157 -> 170 us), as they have to be a tile further ahead.
+//
 // Warps: 0-3 and 4-7 softmax of stage 0 and 1 (a thread per row), 8 issues the MMAs, 9 loads K and V
 // (TMA; E4M3: bulk copies of codes and scales), 10 completes V tiles (rows that nobody sees become
 // zeros), 11 finds the items and loads Q; E4M3 has 12-15 besides, which convert codes to BF16 tiles.
-// TMEM (512 columns): S_0, S_1 (128 columns each; P, as BF16 pairs, over the first 64), O_0, O_1 (128
-// each).  S of a tile goes over P of the one before: the MMAs of one thread run in the order of issue.
+// TMEM (512 columns): the S buffers (128 columns each; P, as BF16 pairs, over the first 64), O_0, O_1.
+// S of a later pair goes over a P: the MMAs of one thread run in the order of issue.
 //
 // Keys that a row does not see have no influence whatever they hold: S is replaced by -inf.  Where V
 // is not finite, P = 0 times V would be NaN; an item whose result is not finite is therefore done
@@ -40,7 +45,7 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9, kCheckWarp = 10, kItemWarp = 11, kCon
 constexpr int kConvWarps = 4;
 constexpr int kConvBatch = 2;  // pieces that a converter thread reads before it writes (1, 2, 4: 257, 241, 247 us)
 constexpr int kBox = kKeys * 128;  // 128 rows x 64 BF16 columns, 128-byte swizzled
-constexpr uint32_t kTmemCols = 512, kTmemS = 0, kTmemO = 256;  // stage s at + 128 s
+constexpr uint32_t kTmemCols = 512;
 constexpr int kRedoBits = 1024;
 
 template <int D, int KV>
@@ -49,10 +54,11 @@ struct ChunkCfg {
   static constexpr int kThreads = kCodes ? 512 : 384;
   // Registers: the launch's threads x registers divided between the softmax warpgroups and the rest
   // (setmaxnreg); the host checks that the kernel was compiled to kLaunchRegs.  9472 tokens over
-  // themselves, 4 heads, BF16: softmax registers 192, 200, 208, 216: 152, 149, 155, 159 us (D 128).
+  // themselves, 4 heads, BF16, softmax registers 192, 200, 208, 216: 152, 149, 155, 159 us (D 128);
+  // 192, 200, 208: 121, 124, 123 us (D 64).
   static constexpr int kLaunchRegs = kCodes ? 128 : 168;
-  static constexpr int kSoftmaxRegs = kCodes ? (D == 128 ? 176 : 184) : 200;
-  static constexpr int kOtherRegs = kCodes ? 256 - kSoftmaxRegs : 104;
+  static constexpr int kSoftmaxRegs = kCodes ? (D == 128 ? 176 : 184) : (D == 128 ? 200 : 192);
+  static constexpr int kOtherRegs = kCodes ? 256 - kSoftmaxRegs : (D == 128 ? 104 : 120);
   static_assert(256 * kSoftmaxRegs + (kThreads - 256) * kOtherRegs <= kThreads * kLaunchRegs,
                 "the register split must fit in what the launch holds");
   static constexpr int kTile = kKeys * D * 2;  // a K, V or stage's Q tile
@@ -60,6 +66,15 @@ struct ChunkCfg {
   static constexpr int kSlots = D == 64 ? 3 : 2;  // K slots = V slots
   static constexpr int kCodeTile = kCodes ? kKeys * D : 0;
   static constexpr int kCodeSlots = kCodes ? (D == 64 ? 4 : 2) : 0;
+  // TMEM: S buffers of 128 columns, which the (tile, stage) pairs take in turn, then O of both stages.
+  static constexpr int kSBufs = D == 64 && !kCodes ? 3 : 2;
+  static constexpr uint32_t kTmemO = 128 * kSBufs, kOStep = kSBufs == 3 ? D : 128;
+  static_assert(kTmemO + 2 * kOStep <= kTmemCols && D <= kOStep, "TMEM of an SM");
+  // With three buffers a stage's next S is done before its P V is, so that two tiles of a stage may be
+  // under way: they take turns on two barriers of each kind, as a wait for one may come two phases late.
+  static constexpr bool kAhead = kSBufs == 3;
+  static __device__ __forceinline__ int turn(int st, int n) { return 2 * st + (kAhead ? n & 1 : 0); }
+  static __device__ __forceinline__ uint32_t phase(int n) { return (uint32_t)(kAhead ? n >> 1 : n) & 1u; }
   static constexpr int kQ = 0;
   static constexpr int kK = kQBufs * 2 * kTile;
   static constexpr int kV = kK + kSlots * kTile;
@@ -67,8 +82,9 @@ struct ChunkCfg {
   static constexpr int kScale = kCode + kCodeSlots * kCodeTile;  // 128 scales per code slot
   static constexpr int kBars = kScale + kCodeSlots * kKeys;
   // Barriers.
-  static constexpr int ITEM_FULL = 0, ITEM_EMPTY = 2, Q_FULL = 4, Q_EMPTY = 6, S_FULL = 8, P_FULL = 10,
-                       PV_DONE = 12, O_FREE = 14, DRAIN = 16, Q_RAW = 17 /* E4M3 */, K_FULL = 19, K_EMPTY = K_FULL + kSlots,
+  static constexpr int ITEM_FULL = 0, ITEM_EMPTY = 2, Q_FULL = 4, Q_EMPTY = 6, S_FULL = 8 /* + turn() */,
+                       P_FULL = 12 /* + turn() */, PV_DONE = 16 /* + turn() */, O_FREE = 20, DRAIN = 22,
+                       Q_RAW = 23 /* E4M3 */, K_FULL = 25, K_EMPTY = K_FULL + kSlots,
                        V_FULL = K_EMPTY + kSlots, V_OK = V_FULL + kSlots, V_EMPTY = V_OK + kSlots,
                        CODE_FULL = V_EMPTY + kSlots, CODE_EMPTY = CODE_FULL + kCodeSlots,
                        NBARS = CODE_EMPTY + kCodeSlots;
@@ -126,7 +142,8 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// The whole warp waits; the vote keeps it together whatever the lanes saw.
+// The whole warp waits, the MMA warp too (its products issued by one thread in a branch of its own took
+// 170 us where the warp's take 160; positions kept in arrays took 260); the vote keeps it together whatever the lanes saw.
 __device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, const Ctl& c) {
   const long long t0 = clock64();
   while (true) {
@@ -260,7 +277,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
       if (i >= C::ITEM_EMPTY && i < C::ITEM_EMPTY + 2) count = 3 + kSoftmaxWarps + (C::kCodes ? kConvWarps - 1 : 0);
       if (i >= C::Q_FULL && i < C::Q_FULL + 2) count = C::kCodes ? kConvWarps : 32;
       if (i >= C::Q_RAW && i < C::Q_RAW + 2) count = 32;
-      if ((i >= C::P_FULL && i < C::P_FULL + 2) || (i >= C::O_FREE && i < C::O_FREE + 2)) count = 4;
+      if ((i >= C::P_FULL && i < C::P_FULL + 4) || (i >= C::O_FREE && i < C::O_FREE + 2)) count = 4;
       if (C::kCodes && ((i >= C::K_FULL && i < C::K_FULL + C::kSlots) || (i >= C::V_OK && i < C::V_OK + C::kSlots)))
         count = kConvWarps;
       if (i >= C::CODE_EMPTY) count = kConvWarps;
@@ -295,8 +312,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
     set_regs_more<C::kSoftmaxRegs>();
     const int st = warp >> 2, quarter = warp & 3;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tS = tmem + kTmemS + 128u * st + lane_base;
-    const uint32_t tO = tmem + kTmemO + 128u * st + lane_base;
+    const uint32_t tO = tmem + C::kTmemO + C::kOStep * (uint32_t)st + lane_base;
     const float sl2 = p.scale_log2;
     int g = 0;   // tiles of this CTA's earlier items (K/V ring position)
     int ns = 0;  // tiles of this stage so far
@@ -336,12 +352,14 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         const int kb = t * kKeys;
         const bool first = !has;
         has = true;
-        if (!waitw(bar(C::S_FULL + st), (uint32_t)ns & 1u, ctl)) {
+        const int turn = C::turn(st, ns);
+        if (!waitw(bar(C::S_FULL + turn), C::phase(ns), ctl)) {
           ok = false;
           break;
         }
         ++ns;
         tc_fence_after();
+        const uint32_t tS = tmem + 128u * ((uint32_t)(2 * (i - c0) + st) % C::kSBufs) + lane_base;
         const bool active = warp_rows && kb <= any_hi && (kb + kKeys > any_lo || kb < p.sinks);
         if (!active) {  // nothing of the tile is seen by these rows
           uint32_t z[32];
@@ -413,7 +431,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           l_run += a0 + a1;
           if (__any_sync(0xffffffffu, need)) {
             // O may be touched once the stage's P V before this tile's has completed.
-            if (!first && !waitw(bar(C::PV_DONE + st), (uint32_t)ns & 1u, ctl)) {
+            if (!first && !waitw(bar(C::PV_DONE + C::turn(st, ns - 2)), C::phase(ns - 2), ctl)) {
               tmem_wait_st();
               ok = false;
               break;
@@ -441,7 +459,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           // V rows that were zeroed for not being finite: add what this row sees of them.
           const int gi = g + i - c0, slot = gi % C::kSlots;
           if (!waitw(bar(C::V_OK + slot), (uint32_t)(gi / C::kSlots) & 1u, ctl) ||
-              (!first && !waitw(bar(C::PV_DONE + st), (uint32_t)ns & 1u, ctl))) {
+              (!first && !waitw(bar(C::PV_DONE + C::turn(st, ns - 2)), C::phase(ns - 2), ctl))) {
             ok = false;
             break;
           }
@@ -484,12 +502,12 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::P_FULL + st));
+        if (lane == 0) mbar_arrive(bar(C::P_FULL + turn));
       }
       if (!ok) break;
       g += c1 - c0;
       // ---- the item's rows: O / l (or the partial O, m, l), then O = 0 for the next item
-      if (has && !waitw(bar(C::PV_DONE + st), (uint32_t)(ns - 1) & 1u, ctl)) break;
+      if (has && !waitw(bar(C::PV_DONE + C::turn(st, ns - 1)), C::phase(ns - 1), ctl)) break;
       tc_fence_after();
       const bool mine_row = wrow + lane < it.rows;
       const bool any = hi >= 0 && (hi >= lo || p.sinks > 0);
@@ -559,7 +577,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
       const uint64_t dK = smem_desc_sw128(sbase + C::kK, 16, 1024);
       const uint64_t dV = smem_desc_sw128(sbase + C::kV, kBox, 1024);
       int g = 0;
-      int np[2] = {0, 0};  // tiles with P V issued, per stage
+      int nq[2] = {0, 0}, np[2] = {0, 0};  // tiles with S and with P V issued, per stage
       int nf[2] = {0, 0};  // items with such tiles, per stage
       bool ok = true;
       for (int k = 0; ok; ++k) {
@@ -570,16 +588,19 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
         if (!waitw(bar(C::Q_FULL + qb), (uint32_t)(k / C::kQBufs) & 1u, ctl)) break;
         fence_proxy_async_smem();  // Q rows were written by cp.async
         const uint64_t dQ = smem_desc_sw128(sbase + C::kQ + (uint32_t)(qb * 2 * C::kTile), 16, 1024);
-        auto issue_s = [&](int s, int gi) {
+        auto issue_s = [&](int s, int i) {
+          const int gi = g + i, buf = (2 * i + s) % C::kSBufs;
+          const uint32_t full = bar(C::S_FULL + C::turn(s, nq[s]));
+          ++nq[s];
           const uint64_t q = dQ + (uint64_t)((s * C::kTile) >> 4);
           const uint64_t kd = dK + (uint64_t)(((gi % C::kSlots) * C::kTile) >> 4);
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint64_t o = (uint64_t)(((kk >> 2) * kBox + (kk & 3) * 32) >> 4);
-              mma_ss(tmem + kTmemS + 128u * s, q + o, kd + o, idS, kk > 0 ? 1u : 0u);
+              mma_ss(tmem + 128u * buf, q + o, kd + o, idS, kk > 0 ? 1u : 0u);
             }
-            mma_commit(bar(C::S_FULL + s));
+            mma_commit(full);
           }
           __syncwarp();
         };
@@ -589,26 +610,40 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
           if (elect_one()) mma_commit(bar(C::Q_EMPTY + qb));
           __syncwarp();
         };
-        if (count > 0) {
-          if (!waitw(bar(C::K_FULL + g % C::kSlots), (uint32_t)(g / C::kSlots) & 1u, ctl)) break;
+        auto wait_k = [&](int i) {
+          const int gi = g + i;
+          if (!waitw(bar(C::K_FULL + gi % C::kSlots), (uint32_t)(gi / C::kSlots) & 1u, ctl)) return false;
           tc_fence_after();
           if (C::kCodes) fence_proxy_async_smem();
+          return true;
+        };
+        auto free_k = [&](int i) {
+          if (elect_one()) mma_commit(bar(C::K_EMPTY + (g + i) % C::kSlots));
+          __syncwarp();
+        };
+        // S is issued kSBufs (tile, stage) pairs ahead of P V.
+        if (count > 0) {
+          if (!wait_k(0)) break;
           const int t = it.all.at(it.c0);
 #pragma unroll
           for (int s = 0; s < 2; ++s)
-            if (needs(it.stage[s], t)) issue_s(s, g);
-          if (elect_one()) mma_commit(bar(C::K_EMPTY + g % C::kSlots));
-          __syncwarp();
+            if (needs(it.stage[s], t)) issue_s(s, 0);
+          free_k(0);
+          if (C::kAhead && count > 1) {
+            if (!wait_k(1)) break;
+            if (needs(it.stage[0], it.all.at(it.c0 + 1))) issue_s(0, 1);
+          }
         }
         if (count <= 1) release_q();
         bool started[2] = {false, false};
         for (int i = 0; i < count; ++i) {
           const int gi = g + i, sl = gi % C::kSlots;
           const int t = it.all.at(it.c0 + i);
-          const bool more = i + 1 < count;
+          // The pairs whose S follows this tile's P V of stage 0 and 1.
+          const bool more = i + 1 < count, more2 = C::kAhead ? i + 2 < count : more;
           const int t1 = more ? it.all.at(it.c0 + i + 1) : 0;
-          if (!waitw(bar(C::V_OK + sl), (uint32_t)(gi / C::kSlots) & 1u, ctl) ||
-              (more && !waitw(bar(C::K_FULL + (gi + 1) % C::kSlots), (uint32_t)((gi + 1) / C::kSlots) & 1u, ctl))) {
+          const int t2 = C::kAhead && more2 ? it.all.at(it.c0 + i + 2) : t1;
+          if (!waitw(bar(C::V_OK + sl), (uint32_t)(gi / C::kSlots) & 1u, ctl) || (!C::kAhead && more && !wait_k(i + 1))) {
             ok = false;
             break;
           }
@@ -628,22 +663,34 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
                 }
                 ++nf[s];
               }
-              if (!waitw(bar(C::P_FULL + s), (uint32_t)np[s] & 1u, ctl)) {
+              if (!waitw(bar(C::P_FULL + C::turn(s, np[s])), C::phase(np[s]), ctl)) {
                 ok = false;
                 break;
               }
+              const uint32_t done = bar(C::PV_DONE + C::turn(s, np[s]));
+              const int buf = (2 * i + s) % C::kSBufs;
               ++np[s];
               tc_fence_after();
               if (elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < kKeys / 16; ++kk)
-                  mma_ts(tmem + kTmemO + 128u * s, tmem + kTmemS + 128u * s + 8u * kk,
+                  mma_ts(tmem + C::kTmemO + C::kOStep * (uint32_t)s, tmem + 128u * buf + 8u * kk,
                          vd + (uint64_t)((kk * 16 * 128) >> 4), idO, 1u);
-                mma_commit(bar(C::PV_DONE + s));
+                mma_commit(done);
               }
               __syncwarp();
             }
-            if (more && needs(it.stage[s], t1)) issue_s(s, gi + 1);
+            if constexpr (!C::kAhead) {
+              if (more && needs(it.stage[s], t1)) issue_s(s, i + 1);
+            } else if (s == 0) {
+              if (more && needs(it.stage[1], t1)) issue_s(1, i + 1);
+            } else if (more2) {
+              if (!wait_k(i + 2)) {
+                ok = false;
+                break;
+              }
+              if (needs(it.stage[0], t2)) issue_s(0, i + 2);
+            }
           }
           if (!ok) break;
           if (elect_one()) {
