@@ -43,7 +43,7 @@ constexpr int kKeys = 128;      // keys of a tile
 constexpr int kSoftmaxWarps = 8;
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kCheckWarp = 10, kItemWarp = 11, kConvWarp0 = 12;
 constexpr int kConvWarps = 4;
-constexpr int kConvBatch = 2;  // pieces that a converter thread reads before it writes (1, 2, 4: 257, 241, 247 us)
+constexpr int kConvBatch = 2;  // pieces that a converter thread has under way (1, 2, 4: 228, 215, 250 us, D 128)
 constexpr int kBox = kKeys * 128;  // 128 rows x 64 BF16 columns, 128-byte swizzled
 constexpr uint32_t kTmemCols = 512;
 constexpr int kRedoBits = 1024;
@@ -981,35 +981,47 @@ __global__ void __launch_bounds__(ChunkCfg<D, KV>::kThreads, 1)
                   wb[x] = lds128v(src + (uint32_t)((r0 + kRowStep * (x0 + x)) * D + 16 * piece));
                   eb[x] = sc[r0 + kRowStep * (x0 + x)];
                 }
+                uint32_t yb[kConvBatch][8];
+                uint32_t top = 0u, most = 0u;  // the largest fields (0x7f0 where a code is NaN) and scale
 #pragma unroll
                 for (int xb = 0; xb < kConvBatch; ++xb) {
-                  const int x = x0 + xb, r = r0 + kRowStep * x;
                   const uint32_t w[4] = {wb[xb].x, wb[xb].y, wb[xb].z, wb[xb].w};
-                  const uint32_t e = eb[xb];
-                  uint32_t y[8];
-                  // value = code fields * 2^120 * 2^(e - 127): one factor where it is a BF16.
-                  uint32_t f = e <= 134u ? (e + 120u) << 7 : 0x7f00u;
-                  f |= f << 16;
-                  uint32_t top = 0u;  // the largest fields: 0x7f0 where a code is NaN
+                  // value = code fields * 2^120 * 2^(e - 127): one factor where it is a BF16 (e <= 134).
+                  const uint32_t f = (min(eb[xb], 134u) + 120u) * 0x00800080u;
+                  most = max(most, eb[xb]);
 #pragma unroll
                   for (int j = 0; j < 4; ++j) {
                     const uint32_t odd = (w[j] >> 4) & 0x07f007f0u, even = (w[j] << 4) & 0x07f007f0u;
                     top = __vimax3_u16x2(top, odd, even);
-                    y[2 * j] = bf16x2_mul(even | ((w[j] << 8) & 0x80008000u), f);
-                    y[2 * j + 1] = bf16x2_mul(odd | (w[j] & 0x80008000u), f);
+                    yb[xb][2 * j] = bf16x2_mul(even | ((w[j] << 8) & 0x80008000u), f);
+                    yb[xb][2 * j + 1] = bf16x2_mul(odd | (w[j] & 0x80008000u), f);
                   }
-                  if (e > 134u || (top >> 16) == 0x7f0u || (top & 0xffffu) == 0x7f0u) {
-                    // (Rare) scales above 2^7, and NaN codes or scale.
+                }
+                if (most > 134u || ((top + 0x00100010u) & 0x08000800u)) {
+                  // (Rare) scales above 2^7, and NaN codes or scale.  One test for the batch: a branch for
+                  // each piece would keep the pieces from overlapping (9472 tokens, 4 heads, D 128: 215
+                  // against 224 us).
+#pragma unroll
+                  for (int xb = 0; xb < kConvBatch; ++xb) {
+                    const uint32_t w[4] = {wb[xb].x, wb[xb].y, wb[xb].z, wb[xb].w};
+                    const uint32_t e = eb[xb];
                     uint32_t f2 = e > 134u && e < 255u ? (e - 7u) << 7 : e == 255u ? 0x7fc0u : 0x3f80u;
                     f2 |= f2 << 16;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                      y[j] = bf16x2_mul(y[j], f2);
+                      uint32_t& y = yb[xb][j];
+                      y = bf16x2_mul(y, f2);
                       const uint32_t two = (j & 1) ? w[j >> 1] >> 8 : w[j >> 1];  // codes in bytes 0 and 2
-                      if ((two & 0x7fu) == 0x7fu) y[j] = (y[j] & 0xffff0000u) | 0x7fc0u;
-                      if ((two & 0x7f0000u) == 0x7f0000u) y[j] = (y[j] & 0xffffu) | 0x7fc00000u;
+                      if ((two & 0x7fu) == 0x7fu) y = (y & 0xffff0000u) | 0x7fc0u;
+                      if ((two & 0x7f0000u) == 0x7f0000u) y = (y & 0xffffu) | 0x7fc00000u;
                     }
                   }
+                }
+#pragma unroll
+                for (int xb = 0; xb < kConvBatch; ++xb) {
+                  const int x = x0 + xb;
+                  [[maybe_unused]] const int r = r0 + kRowStep * x;
+                  uint32_t (&y)[8] = yb[xb];
                   if constexpr (!decltype(plain)::value) {
                     if (unseen(it, p.sinks, kb + r)) {
 #pragma unroll
