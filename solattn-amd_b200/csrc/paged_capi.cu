@@ -144,7 +144,9 @@ Choice choose(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   const int64_t most = paged ? (most_new > 0 && most_new < N ? most_new : N) * G : Tq * G;
   const int64_t mean = paged ? N * G / B : Tq * G;
   c.many = most >= kManyRows;
-  c.few = mean < kManyRows;
+  // (Rows behind the last sequence raise the mean, and most_new is a hint: one of the two always runs, and
+  // each alone does whatever the sequences hold.)
+  c.few = mean < kManyRows || !c.many;
   c.rows = rows_split(N, B, Hq, Hkv, Tq, c.many ? kManyRows : most, cap, paged, r);
   c.chunk = chunk_split(N, B, Hq, Hkv, Tq, cap, paged, r);
   c.rows_bytes = c.few ? split_bytes(c.rows, c.rows.rows, Hkv, D) : 0;

@@ -426,3 +426,22 @@ def test_offsets_past_32_bits(new):
     rk, rv = cache_read(cache, plan, L)
     assert torch.equal(rk[0].cpu(), x) and torch.equal(rv[0].cpu(), y)
     check_device_errors()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("behind", [0, 400])
+@pytest.mark.parametrize("hint", [0, 1, 3, 200, 1000])
+@pytest.mark.parametrize("counts", [[(1, 300)], [(3, 200), (1, 50)], [(200, 400), (1, 30), (0, 9)]])
+def test_paged_attention_hints_and_padding(kind, behind, hint, counts):
+    """most_new chooses kernels only, right or wrong, with many rows behind the last sequence too."""
+    s = Sequences(counts, heads=2, dim=64, page=16, kind=kind)
+    q = s.queries(4, 64, rows=s.tokens + behind)
+    plan = PagedPlan(s.plan.page_table, s.plan.key_lengths, s.plan.query_starts, hint)
+    expected, tolerance = s.expected(q)
+    out = paged_attention(to_device(q), s.cache, plan)
+    assert_within(out[:s.tokens], expected, tolerance)
+    assert not out[s.tokens:].any()
+    kept = torch.full_like(out, 7.0)
+    paged_attention(to_device(q), s.cache, plan, out=kept)
+    assert torch.equal(kept[:s.tokens], out[:s.tokens]) and bool((kept[s.tokens:] == 7.0).all())
+    check_device_errors()
