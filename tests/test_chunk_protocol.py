@@ -44,7 +44,7 @@ def run(items, again, ahead, slots, qbufs, codes, seed):
 
     for j in range(2):
         bar(f"IF{j}")
-        bar(f"IE{j}", 10 + (1 if codes else 1))  # MMA, loader, checker or converters, 8 softmax warps
+        bar(f"IE{j}", 11)  # MMA, loader, V checker or converters, 8 softmax warps
         bar(f"QF{j}")
         bar(f"QR{j}")
         bar(f"QE{j}")
@@ -131,7 +131,7 @@ def run(items, again, ahead, slots, qbufs, codes, seed):
                     yield ("do", lambda land=land: copies.append(land))
                 g += 1
 
-    def checker():
+    def v_checker():
         g = 0
         for k, it in enumerate(order):
             yield from take(k)
@@ -314,7 +314,7 @@ def run(items, again, ahead, slots, qbufs, codes, seed):
                 let_go(k)
             yield ("do", end)
 
-    roles = [item_warp(), loader(), converter() if codes else checker(), mma_warp()]
+    roles = [item_warp(), loader(), converter() if codes else v_checker(), mma_warp()]
     roles += [softmax(st, w) for st in range(2) for w in range(4)]
     state = [next(r, None) for r in roles]
     weights = [rng.choice((1, 1, 4, 20)) for _ in roles]
