@@ -19,6 +19,7 @@ using namespace solattn;
 namespace {
 
 constexpr int64_t kMaxKeys = int64_t(1) << 24;  // keys of a sequence, as in the routed entry points
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 4096;  // (token, head) rows of a K/V head: with a tile, an int
 constexpr int64_t kSms = 148;
 
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -164,7 +165,7 @@ int check_window(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hkv, int
   const int rc = check_heads(Hq, Hkv, D);
   if (rc) return rc;
   if (!rule_ok(r) || Tq > kMaxKeys || Tk > kMaxKeys) return SOLATTN_ERR_ARG;
-  if (B * Tq > (int64_t(1) << 31) / (Hq / Hkv) - 1 || B > (1 << 24)) return SOLATTN_ERR_ARG;
+  if (B > (1 << 24) || B * Tq > kMaxRows / (Hq / Hkv)) return SOLATTN_ERR_ARG;
   return SOLATTN_OK;
 }
 int check_paged(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t page_size, int64_t width,
@@ -174,7 +175,7 @@ int check_paged(int64_t N, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_
   if (rc) return rc;
   if (page_shift_of(page_size) < 0) return SOLATTN_ERR_UNSUPPORTED;
   if (!rule_ok(r) || width * page_size > kMaxKeys) return SOLATTN_ERR_ARG;
-  if (N > (int64_t(1) << 31) / (Hq / Hkv) - 1 - (1 << 24) || B > (1 << 24)) return SOLATTN_ERR_ARG;
+  if (N > kMaxRows / (Hq / Hkv) || B > (1 << 24)) return SOLATTN_ERR_ARG;
   return SOLATTN_OK;
 }
 

@@ -173,3 +173,14 @@ def test_workspace_sizes():
     assert size > 0 and size % (8 * 130 * 4) == 0
     # A window bounds what is split, however wide the table is.
     assert L.solattn_paged_workspace_bytes(1, 1, 16, 2, 128, 64, 1 << 18, 1, 64, 0, 4) == 0
+
+
+@pytest.mark.parametrize("group", [1, 127, 128, 129, 1000, 65535])
+def test_row_limits(group):
+    """(token, head) rows are counted in 32 bits; any number of heads may share K and V."""
+    lib = _lib.load()
+    most = (2 ** 31 - 4096) // group
+    for n, fine in ((1, True), (most, True), (most + 1, False)):
+        got = lib.solattn_paged_workspace_bytes(n, 1, group, 1, 64, 16, 8, 0, 0, 0, 0)
+        assert (got >= 0) == fine, n
+    assert lib.solattn_window_workspace_bytes(1, 1, 100, group, 1, 64, 0, 0, 0) >= 0

@@ -445,3 +445,16 @@ def test_paged_attention_hints_and_padding(kind, behind, hint, counts):
     paged_attention(to_device(q), s.cache, plan, out=kept)
     assert torch.equal(kept[:s.tokens], out[:s.tokens]) and bool((kept[s.tokens:] == 7.0).all())
     check_device_errors()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("heads", [95, 128, 300])
+def test_many_query_heads_of_one_kv_head(kind, heads):
+    """One new token is many rows where the heads share K and V."""
+    s = Sequences([(1, 300), (2, 70), (0, 5), (1, 1)], heads=1, dim=64, page=16, kind=kind)
+    q = s.queries(heads, 64)
+    for rule in (dict(), dict(window=33, sink_tokens=3)):
+        assert_within(paged_attention(to_device(q), s.cache, s.plan, **rule), *s.expected(q, **rule))
+    check_device_errors()
+    if kind == "bf16":
+        _check_window(*_bthd(2, 1, 300, heads, 1, 64), window=100)
