@@ -125,7 +125,7 @@ def _launch(q, k, v, rule, scale, shape, strides):
     device = q.device
     word = error_word(device.index)  # an earlier call's device-side error surfaces here
     keep, ws, size = workspace("solattn_window_workspace_bytes", shape + rule, device)
-    out = torch.empty(q.shape, dtype=torch.bfloat16, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     rc = _lib.load().solattn_window_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, *strides, *rule, scale, ws, size, out.data_ptr(),
         word, current_stream(device.index))
