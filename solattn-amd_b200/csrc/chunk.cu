@@ -55,7 +55,8 @@ struct ChunkCfg {
   // Registers: the launch's threads x registers divided between the softmax warpgroups and the rest
   // (setmaxnreg); the host checks that the kernel was compiled to kLaunchRegs.  9472 tokens over
   // themselves, 4 heads, BF16, softmax registers 192, 200, 208, 216: 152, 149, 155, 159 us (D 128);
-  // 192, 200, 208: 121, 124, 123 us (D 64).
+  // 192, 200, 208: 121, 124, 123 us (D 64).  E4M3, 160, 168, 176, 184: 216, 215, 214, 217 us (D 128); 168, 176,
+  // 184, 192: 169, 166, 165, 169 us (D 64).
   static constexpr int kLaunchRegs = kCodes ? 128 : 168;
   static constexpr int kSoftmaxRegs = kCodes ? (D == 128 ? 176 : 184) : (D == 128 ? 200 : 192);
   static constexpr int kOtherRegs = kCodes ? 256 - kSoftmaxRegs : (D == 128 ? 104 : 120);
@@ -142,8 +143,8 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// The whole warp waits, the MMA warp too (its products issued by one thread in a branch of its own took
-// 170 us where the warp's take 160; positions kept in arrays took 260); the vote keeps it together whatever the lanes saw.
+// The whole warp waits; the vote keeps it together whatever the lanes saw.  (The MMA warp too: its products
+// issued by one thread in a branch of its own took 170 us where the warp's take 160.)
 __device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, const Ctl& c) {
   const long long t0 = clock64();
   while (true) {
